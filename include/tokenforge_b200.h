@@ -313,6 +313,56 @@ TF_API int tf_e4m3_quant_rows(const uint16_t* y, int64_t R, int64_t C, int64_t l
                               const float* scale, int64_t scale_stride, uint8_t* q,
                               float* scale_out, void* stream);
 
+/* ------------------------------------------------- FP8 block-scaled (W8A8) linear path
+ * e4m3 activations with one fp32 scale per row and 128 columns, e4m3 weights with one fp32
+ * scale per 128 x 128 block (the layout of block-quantized FP8 checkpoints). No reference
+ * counterpart: the reference's e4m3 output has no consumer and its weights are int4.
+ *
+ * Streams and outputs are fp16 or bf16 (`dtype`), passed as 16-bit patterns. The quantizers
+ * below write q contiguous [rows, columns] and scale_out contiguous: [rows, ceil(columns /
+ * 128)] with group_size 128, [rows] with group_size 0 (one scale per row, the form
+ * tf_w4a16_linear_fp8 takes). The last group of a row may be shorter. The rule of each group:
+ *   scale = max(amax|y| / 448, 1 / (448 * 512)),  q = e4m3_rne_satfinite(y / scale),
+ * y in fp32, never rounded to the stream's type. A NaN in a group makes its scale and all its
+ * codes NaN; an infinite value makes the scale infinite, its own code NaN and the others 0.
+ * Rows need not be aligned and row strides may be any number of elements >= the row; 16-byte
+ * aligned rows whose stride and length are multiples of 8 elements run several times faster. */
+enum { TF_DTYPE_FP16 = 0, TF_DTYPE_BF16 = 1 };
+
+/* residual_out = dtype(x + residual);  h = residual_out in fp32;
+ * y = h * (1 / sqrt(mean(h^2) + eps)) * weight.
+ * residual may be NULL (then residual_out must be NULL and h = x). residual_out may be residual
+ * itself or x itself; no other overlap of an output with an operand is allowed. */
+TF_API int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t T, int64_t H, int64_t ldx,
+                                    const uint16_t* residual, int64_t ldr,
+                                    const uint16_t* weight, float eps, int32_t dtype,
+                                    int32_t group_size, uint8_t* q, float* scale_out,
+                                    uint16_t* residual_out, int64_t ldo, void* stream);
+
+/* y = silu(gate_up[:, :I]) * gate_up[:, I:], silu(g) = g / (1 + exp(-g)). */
+TF_API int tf_silu_mul_fp8_quant(const uint16_t* gate_up, int64_t M, int64_t I, int64_t ld,
+                                 int32_t dtype, int32_t group_size, uint8_t* q,
+                                 float* scale_out, void* stream);
+
+/* y = x, a scale per 128 columns; the codes are those of the IEEE fp32 division. */
+TF_API int tf_e4m3_quant_groups(const uint16_t* x, int64_t R, int64_t C, int64_t ldx,
+                                int32_t dtype, uint8_t* q, float* scale_out, void* stream);
+
+/* y[m, n] = sum_b x_scale[m, b] * w_scale[n / 128, b] * sum_{k in block b} xq[m, k] * wq[n, k]
+ *           (+ bias[n]),  b over the 128-wide blocks of K; fp32 sums, one rounding to dtype.
+ * xq [M, K] row stride ldx bytes; x_scale [M, ceil(K / 128)] row stride ld_xs floats;
+ * wq [N, K] contiguous; w_scale [ceil(N / 128), ceil(K / 128)] contiguous; bias dtype [N] or
+ * NULL; y dtype [M, N] row stride ldy. K and ldx must be multiples of 16, xq and wq 16-byte
+ * aligned; any M >= 0 and N >= 1. Workspace: tf_w8a8_workspace_bytes(M, N, K) bytes, 16-byte
+ * aligned (may be 0, then NULL); it need not be initialised and must not be shared with a call
+ * that runs concurrently. Results do not depend on timing: the same call gives the same bits. */
+TF_API size_t tf_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+TF_API int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
+                                const float* x_scale, int64_t ld_xs, const uint8_t* wq,
+                                const float* w_scale, const uint16_t* bias, int64_t N,
+                                int32_t dtype, uint16_t* y, int64_t ldy, void* workspace,
+                                size_t workspace_bytes, void* stream);
+
 /* Device-side status word written by kernels whose waits are bounded: 0 = no error; 0x1xx the
  * tcgen05 GEMM (a pipeline wait gave up), 0x301 the RMSNorm + FP8 streaming kernel (a row's
  * bulk copy did not complete in time). Reading it synchronises the current device; resetting

@@ -26,6 +26,9 @@ TF_ERR_TOO_LARGE = 7
 
 TF_LAUNCH_PDL = 1
 
+TF_DTYPE_FP16 = 0
+TF_DTYPE_BF16 = 1
+
 _P = ctypes.c_void_p
 _I64 = ctypes.c_int64
 _I32 = ctypes.c_int32
@@ -91,6 +94,17 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "tf_rmsnorm_fp8_quant": (ctypes.c_int, [_P, _I64, _I64, _I64, _P, _F32, _P, _P, _P, _P]),
     "tf_cast_e4m3": (ctypes.c_int, [_P, _I64, _P, _P]),
     "tf_e4m3_quant_rows": (ctypes.c_int, [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P]),
+    "tf_add_rmsnorm_fp8_quant": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _F32, _I32, _I32, _P, _P, _P, _I64, _P],
+    ),
+    "tf_silu_mul_fp8_quant": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _I32, _P, _P, _P]),
+    "tf_e4m3_quant_groups": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _P]),
+    "tf_w8a8_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
+    "tf_w8a8_block_linear": (
+        ctypes.c_int,
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _P, _I64, _P, _SZ, _P],
+    ),
     "tf_device_error": (ctypes.c_int, [_P]),
     "tf_reset_device_error": (ctypes.c_int, []),
     "tf_decode_chain_create": (ctypes.c_int, [_P, _I32, _I64, _I32, _P]),
@@ -187,6 +201,17 @@ def check(fn: str, status: int) -> None:
 def stream_ptr(device: torch.device) -> int:
     """Raw handle of the current CUDA stream on ``device`` (work is enqueued there)."""
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def call_on(device: torch.device, fn, *args) -> int:  # type: ignore[no-untyped-def]
+    """``fn(*args, stream)`` with ``device`` current and its current stream's handle, switching
+    devices only where another one is current: the launch path of the short operators, whose
+    calls cost the host more than the GPU."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return fn(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

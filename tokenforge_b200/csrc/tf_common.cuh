@@ -23,7 +23,7 @@ inline int check_launch() {
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
-inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
+__host__ __device__ constexpr int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Offset j (0..7) of a packed word lives in nibble (j % 2) * 4 + j / 2 (the AWQ interleave,
 // reference tokenforge/kernels/pack.py:35).

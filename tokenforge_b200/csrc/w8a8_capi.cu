@@ -1,0 +1,32 @@
+// C ABI of the block-scaled FP8 linear: argument checks and the choice of kernel.
+#include "tf_common.cuh"
+#include "tf_plan.h"
+#include "tf_w8a8.h"
+
+using namespace tfb;
+
+extern "C" size_t tf_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  (void)M;
+  (void)N;
+  (void)K;
+  return 0;
+}
+
+extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
+                                    const float* x_scale, int64_t ld_xs, const uint8_t* wq,
+                                    const float* w_scale, const uint16_t* bias, int64_t N,
+                                    int32_t dtype, uint16_t* y, int64_t ldy, void* workspace,
+                                    size_t workspace_bytes, void* stream) {
+  (void)workspace;
+  (void)workspace_bytes;
+  if (M < 0 || N < 1 || K < 1 || (dtype != TF_DTYPE_FP16 && dtype != TF_DTYPE_BF16))
+    return TF_ERR_INVALID_ARG;
+  if (K % 16 != 0) return TF_ERR_UNSUPPORTED;
+  if (M == 0) return TF_OK;
+  if (!xq || !x_scale || !wq || !w_scale || !y || ldx < K || ld_xs < cdiv(K, 128) || ldy < N)
+    return TF_ERR_INVALID_ARG;
+  if (!aligned16(xq) || !aligned16(wq) || ldx % 16 != 0) return TF_ERR_ALIGNMENT;
+  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL) return TF_ERR_TOO_LARGE;
+  const W8A8Args a{xq, x_scale, wq, w_scale, bias, y, M, N, K, ldx, ld_xs, ldy, dtype};
+  return launch_w8a8_gemv(a, static_cast<cudaStream_t>(stream));
+}

@@ -8,6 +8,8 @@ tensor values, shape-only dispatch), plus ``tokenforge::awq_repack``:
 * ``tokenforge::w4a16_dequant(qweight_t, scales, qzeros, group_size) -> w [N, K] fp16``
 * ``tokenforge::rmsnorm_fp8_quant(x, weight, eps, scale) -> (q e4m3, scale fp32)``
 * ``tokenforge::awq_repack(qweight) -> qweight_t``
+* the FP8 block-scaled path (``tokenforge_b200.fp8``): ``tokenforge::w8a8_block_linear``,
+  ``add_rmsnorm_fp8_quant``, ``silu_mul_fp8_quant``, ``e4m3_quant_groups``
 
 Every real implementation enqueues kernels on the current CUDA stream through the C ABI; the
 only allocations are outputs and the optional split-K workspace, both from PyTorch's caching
@@ -21,6 +23,13 @@ import functools
 import torch
 
 from tokenforge_b200 import _lib, dispatch
+from tokenforge_b200.fp8 import GROUP as FP8_GROUP
+from tokenforge_b200.fp8 import (  # noqa: F401  (re-exported launch API)
+    add_rmsnorm_fp8_quant,
+    e4m3_quant_groups,
+    silu_mul_fp8_quant,
+    w8a8_block_linear,
+)
 from tokenforge_b200.linear import (  # noqa: F401  (re-exported launch API)
     _VEC,
     _aligned_rows,
@@ -510,3 +519,75 @@ def e4m3_quant_rows(y: torch.Tensor, scale: torch.Tensor | None = None
             s_out.data_ptr() if scale is None else None, _lib.stream_ptr(y.device))
     _lib.check("tf_e4m3_quant_rows", status)
     return out, s_out
+
+
+# ------------------------------------------------------------- FP8 block-scaled (W8A8) path
+#
+# tokenforge_b200.fp8 holds the launchers, exported here for direct calls; the registrations
+# below give the same operators to traced programs (a custom op may not return its input, so
+# without a residual the registered norm returns a copy of x).
+
+
+@torch.library.custom_op("tokenforge::w8a8_block_linear", mutates_args=())
+def _w8a8_block_linear_op(
+    xq: torch.Tensor,
+    x_scale: torch.Tensor,
+    wq: torch.Tensor,
+    w_scale: torch.Tensor,
+    bias: torch.Tensor | None,
+    out_dtype: torch.dtype,
+) -> torch.Tensor:
+    return w8a8_block_linear(xq, x_scale, wq, w_scale, bias, out_dtype)
+
+
+@_w8a8_block_linear_op.register_fake
+def _w8a8_block_linear_fake(xq, x_scale, wq, w_scale, bias, out_dtype):  # type: ignore[no-untyped-def]
+    return torch.empty((*xq.shape[:-1], wq.shape[0]), dtype=out_dtype, device=xq.device)
+
+
+@torch.library.custom_op("tokenforge::add_rmsnorm_fp8_quant", mutates_args=())
+def _add_rmsnorm_fp8_quant_op(
+    x: torch.Tensor,
+    residual: torch.Tensor | None,
+    weight: torch.Tensor,
+    eps: float,
+    group_size: int,
+) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    q, s, total = add_rmsnorm_fp8_quant(x, residual, weight, eps, group_size)
+    return q, s, total.clone() if residual is None else total
+
+
+def _group_scales(x, columns, group_size):  # type: ignore[no-untyped-def]
+    groups = -(-columns // FP8_GROUP) if group_size else 1
+    return x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
+
+
+@_add_rmsnorm_fp8_quant_op.register_fake
+def _add_rmsnorm_fp8_quant_fake(x, residual, weight, eps, group_size):  # type: ignore[no-untyped-def]
+    q = x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
+    return q, _group_scales(x, x.shape[-1], group_size), x.new_empty(x.shape)
+
+
+@torch.library.custom_op("tokenforge::silu_mul_fp8_quant", mutates_args=())
+def _silu_mul_fp8_quant_op(
+    gate_up: torch.Tensor, group_size: int
+) -> tuple[torch.Tensor, torch.Tensor]:
+    return silu_mul_fp8_quant(gate_up, group_size)
+
+
+@_silu_mul_fp8_quant_op.register_fake
+def _silu_mul_fp8_quant_fake(gate_up, group_size):  # type: ignore[no-untyped-def]
+    i = gate_up.shape[-1] // 2
+    q = gate_up.new_empty((*gate_up.shape[:-1], i), dtype=torch.float8_e4m3fn)
+    return q, _group_scales(gate_up, i, group_size)
+
+
+@torch.library.custom_op("tokenforge::e4m3_quant_groups", mutates_args=())
+def _e4m3_quant_groups_op(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return e4m3_quant_groups(x)
+
+
+@_e4m3_quant_groups_op.register_fake
+def _e4m3_quant_groups_fake(x):  # type: ignore[no-untyped-def]
+    return (x.new_empty(x.shape, dtype=torch.float8_e4m3fn),
+            _group_scales(x, x.shape[-1], FP8_GROUP))

@@ -160,3 +160,53 @@ def awq_dequantize(
 ) -> torch.Tensor:
     """AWQ format -> fp16 ``[K, N]`` with the single-rounding dequant rule."""
     return dequantize_tf(pack_awq(qweight, qzeros, scales, group_size)).t()
+
+
+# ----------------------------------------------------------------------- FP8 block scales
+
+FP8_BLOCK = 128
+FP8_MAX = 448.0
+FP8_MIN_SCALE = 1.0 / (448.0 * 512.0)
+
+
+@dataclass(frozen=True)
+class W8A8BlockWeights:
+    """One linear layer in e4m3 with a scale per 128 x 128 block, as block-quantized FP8
+    checkpoints hold it: ``w[n, k] = wq[n, k] * w_scale[n // 128, k // 128]``."""
+
+    wq: torch.Tensor  # float8_e4m3fn [N, K]
+    w_scale: torch.Tensor  # fp32 [ceil(N / 128), ceil(K / 128)]
+
+    @property
+    def n(self) -> int:
+        return self.wq.shape[0]
+
+    @property
+    def k(self) -> int:
+        return self.wq.shape[1]
+
+    def to(self, device: torch.device | str) -> W8A8BlockWeights:
+        return W8A8BlockWeights(self.wq.to(device), self.w_scale.to(device))
+
+
+def pack_w8a8_block(weight: torch.Tensor) -> W8A8BlockWeights:
+    """Load-time conversion of ``nn.Linear.weight`` [N, K] (fp16, bf16 or fp32) with the
+    activations' rule per block: scale = max(amax / 448, 1 / (448 * 512)), e4m3(w / scale)."""
+    if weight.dim() != 2 or 0 in weight.shape:
+        raise ValueError(f"weight must be [N, K] with N, K >= 1, got {tuple(weight.shape)}")
+    if weight.dtype not in (torch.float16, torch.bfloat16, torch.float32):
+        raise TypeError(f"weight must be fp16, bf16 or fp32, got {weight.dtype}")
+    n, k = weight.shape
+    nb, kb = -(-n // FP8_BLOCK), -(-k // FP8_BLOCK)
+    w = torch.zeros((nb * FP8_BLOCK, kb * FP8_BLOCK), dtype=torch.float32, device=weight.device)
+    w[:n, :k] = weight
+    w = w.view(nb, FP8_BLOCK, kb, FP8_BLOCK)
+    scale = (w.abs().amax(dim=(1, 3)) / FP8_MAX).clamp(min=FP8_MIN_SCALE)
+    q = (w / scale[:, None, :, None]).clamp(-FP8_MAX, FP8_MAX).to(torch.float8_e4m3fn)
+    return W8A8BlockWeights(q.view(nb * FP8_BLOCK, kb * FP8_BLOCK)[:n, :k].contiguous(), scale)
+
+
+def dequantize_w8a8_block(weights: W8A8BlockWeights) -> torch.Tensor:
+    """fp32 ``[N, K]`` of the block-scaled weights (torch; load-time and test use)."""
+    s = weights.w_scale.repeat_interleave(FP8_BLOCK, dim=0)[: weights.n]
+    return weights.wq.float() * s.repeat_interleave(FP8_BLOCK, dim=1)[:, : weights.k]
