@@ -365,7 +365,8 @@ TF_API int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t
 
 /* Device-side status word written by kernels whose waits are bounded: 0 = no error; 0x1xx the
  * tcgen05 GEMM (a pipeline wait gave up), 0x301 the RMSNorm + FP8 streaming kernel (a row's
- * bulk copy did not complete in time). Reading it synchronises the current device; resetting
+ * bulk copy did not complete in time), 0x4xx the block-scaled FP8 GEMM (a pipeline wait gave
+ * up). Reading it synchronises the current device; resetting
  * writes 0. */
 TF_API int tf_device_error(int* out_code);
 TF_API int tf_reset_device_error(void);

@@ -38,6 +38,9 @@ uint32_t launch_flags();
 // Status word of the RMSNorm streaming kernel's bounded waits (rmsnorm_fp8.cu).
 int rms_device_error(int* code);
 int rms_reset_device_error();
+// Status word of the block-scaled FP8 GEMM's bounded waits (w8a8_gemm_sm100.cu).
+int w8a8_device_error(int* code);
+int w8a8_reset_device_error();
 
 struct LinearArgs {
   const uint16_t* x;

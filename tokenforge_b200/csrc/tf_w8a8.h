@@ -19,5 +19,6 @@ struct W8A8Args {
 };
 
 int launch_w8a8_gemv(const W8A8Args& a, cudaStream_t stream);
+int launch_w8a8_tc(const W8A8Args& a, cudaStream_t stream);
 
 }  // namespace tfb

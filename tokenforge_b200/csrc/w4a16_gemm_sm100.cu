@@ -33,6 +33,7 @@
 #include "tf_async.cuh"
 #include "tf_common.cuh"
 #include "tf_plan.h"
+#include "tf_tcgen05.cuh"
 
 namespace tfb {
 
@@ -141,26 +142,6 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int si
   return mbar_wait_slow(bar, parity, site);
 }
 
-__device__ __forceinline__ void tc_fence_before() {
-  asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-}
-__device__ __forceinline__ void tc_fence_after() {
-  asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t* slot, uint32_t ncols) {
-  asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
-                   smem_u32(slot)),
-               "r"(ncols)
-               : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-  asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols)
-               : "memory");
-}
-
 // D[tmem] (+)= A[smem] * B[smem]^T, fp16 inputs, fp32 accumulate, issued by one thread.
 __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
                                          uint32_t idesc, uint32_t accumulate) {
@@ -170,53 +151,6 @@ __device__ __forceinline__ void umma_f16(uint32_t d_tmem, uint64_t a_desc, uint6
       "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
       "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
       : "memory");
-}
-
-// Arrive on `bar` once every tcgen05 operation issued so far by this thread has completed.
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-  asm volatile(
-      "tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(
-          smem_u32(bar))
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_ld_32cols(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
-        "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
-        "=r"(r[31])
-      : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_ld_16cols(uint32_t taddr, uint32_t (&r)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
-        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]),
-        "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-      : "r"(taddr));
-}
-
-__device__ __forceinline__ void tmem_ld_wait() {
-  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-}
-
-// Shared-memory matrix descriptor of a K-major tile with the 128-byte swizzle: rows of 128 bytes,
-// 8-row core groups 1024 bytes apart (stride byte offset), descriptor version 1, layout type 2.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr) {
-  uint64_t d = static_cast<uint64_t>((saddr >> 4) & 0x3FFFu);
-  d |= static_cast<uint64_t>(1) << 16;          // leading byte offset (unused when swizzled)
-  d |= static_cast<uint64_t>(1024 >> 4) << 32;  // stride byte offset
-  d |= static_cast<uint64_t>(1) << 46;          // version
-  d |= static_cast<uint64_t>(2) << 61;          // SWIZZLE_128B
-  return d;
 }
 
 // Instruction descriptor: fp16 A and B, fp32 D, both K-major, M = 128, N = BM.
@@ -801,7 +735,8 @@ int launch_tc_gemm(const LinearPlan& pl, const LinearArgs& a, cudaStream_t strea
 
 }  // namespace tfb
 
-// The GEMM's status word first (0x1xx codes), else the RMSNorm streaming kernel's (0x3xx).
+// The GEMM's status word first (0x1xx codes), else the RMSNorm streaming kernel's (0x3xx), else
+// the block-scaled FP8 GEMM's (0x4xx).
 extern "C" int tf_device_error(int* out_code) {
   if (!out_code) return TF_ERR_INVALID_ARG;
   const cudaError_t e = cudaMemcpyFromSymbol(out_code, tfb::g_device_error, sizeof(int));
@@ -809,7 +744,9 @@ extern "C" int tf_device_error(int* out_code) {
     tfb::last_cuda_error() = static_cast<int>(e);
     return TF_ERR_CUDA;
   }
-  return *out_code != 0 ? TF_OK : tfb::rms_device_error(out_code);
+  if (*out_code != 0) return TF_OK;
+  const int st = tfb::rms_device_error(out_code);
+  return st != TF_OK || *out_code != 0 ? st : tfb::w8a8_device_error(out_code);
 }
 
 extern "C" int tf_reset_device_error(void) {
@@ -819,5 +756,6 @@ extern "C" int tf_reset_device_error(void) {
     tfb::last_cuda_error() = static_cast<int>(e);
     return TF_ERR_CUDA;
   }
-  return tfb::rms_reset_device_error();
+  const int st = tfb::rms_reset_device_error();
+  return st != TF_OK ? st : tfb::w8a8_reset_device_error();
 }

@@ -28,5 +28,6 @@ extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int
   if (!aligned16(xq) || !aligned16(wq) || ldx % 16 != 0) return TF_ERR_ALIGNMENT;
   if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL) return TF_ERR_TOO_LARGE;
   const W8A8Args a{xq, x_scale, wq, w_scale, bias, y, M, N, K, ldx, ld_xs, ldy, dtype};
-  return launch_w8a8_gemv(a, static_cast<cudaStream_t>(stream));
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  return M <= 8 ? launch_w8a8_gemv(a, s) : launch_w8a8_tc(a, s);
 }
