@@ -353,15 +353,12 @@ TF_API int tf_e4m3_quant_groups(const uint16_t* x, int64_t R, int64_t C, int64_t
  * xq [M, K] row stride ldx bytes; x_scale [M, ceil(K / 128)] row stride ld_xs floats;
  * wq [N, K] contiguous; w_scale [ceil(N / 128), ceil(K / 128)] contiguous; bias dtype [N] or
  * NULL; y dtype [M, N] row stride ldy. K and ldx must be multiples of 16, xq and wq 16-byte
- * aligned; any M >= 0 and N >= 1. Workspace: tf_w8a8_workspace_bytes(M, N, K) bytes, 16-byte
- * aligned (may be 0, then NULL); it need not be initialised and must not be shared with a call
- * that runs concurrently. Results do not depend on timing: the same call gives the same bits. */
-TF_API size_t tf_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ * aligned; any M >= 0 and N >= 1. No workspace; results do not depend on timing: the same call
+ * gives the same bits. */
 TF_API int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
                                 const float* x_scale, int64_t ld_xs, const uint8_t* wq,
                                 const float* w_scale, const uint16_t* bias, int64_t N,
-                                int32_t dtype, uint16_t* y, int64_t ldy, void* workspace,
-                                size_t workspace_bytes, void* stream);
+                                int32_t dtype, uint16_t* y, int64_t ldy, void* stream);
 
 /* Device-side status word written by kernels whose waits are bounded: 0 = no error; 0x1xx the
  * tcgen05 GEMM (a pipeline wait gave up), 0x301 the RMSNorm + FP8 streaming kernel (a row's

@@ -157,7 +157,7 @@ def test_pack_refusals_and_zero_blocks() -> None:
 
 def _abi_linear(m=1, k=128, ldx=128, ldxs=1, n=128, dtype=0, ldy=128, xq=16, wq=16, y=16):  # type: ignore[no-untyped-def]
     return _lib.lib().tf_w8a8_block_linear(xq, m, k, ldx, 16, ldxs, wq, 16, None, n, dtype, y, ldy,
-                                           None, 0, None)
+                                           None)
 
 
 @pytest.mark.parametrize(

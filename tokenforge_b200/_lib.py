@@ -100,10 +100,9 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
     ),
     "tf_silu_mul_fp8_quant": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _I32, _P, _P, _P]),
     "tf_e4m3_quant_groups": (ctypes.c_int, [_P, _I64, _I64, _I64, _I32, _P, _P, _P]),
-    "tf_w8a8_workspace_bytes": (_SZ, [_I64, _I64, _I64]),
     "tf_w8a8_block_linear": (
         ctypes.c_int,
-        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _P, _I64, _P, _SZ, _P],
+        [_P, _I64, _I64, _I64, _P, _I64, _P, _P, _P, _I64, _I32, _P, _I64, _P],
     ),
     "tf_device_error": (ctypes.c_int, [_P]),
     "tf_reset_device_error": (ctypes.c_int, []),
@@ -203,11 +202,10 @@ def stream_ptr(device: torch.device) -> int:
     return torch.cuda.current_stream(device).cuda_stream
 
 
-def call_on(device: torch.device, fn, *args) -> int:  # type: ignore[no-untyped-def]
-    """``fn(*args, stream)`` with ``device`` current and its current stream's handle, switching
-    devices only where another one is current: the launch path of the short operators, whose
-    calls cost the host more than the GPU."""
-    index = device.index
+def call_on(index: int, fn, *args) -> int:  # type: ignore[no-untyped-def]
+    """``fn(*args, stream)`` with CUDA device ``index`` current and its current stream's handle,
+    switching devices only where another one is current: the launch path of the short operators,
+    whose calls cost the host more than the GPU."""
     if index == torch._C._cuda_getDevice():
         return fn(*args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):

@@ -5,20 +5,10 @@
 
 using namespace tfb;
 
-extern "C" size_t tf_w8a8_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  (void)M;
-  (void)N;
-  (void)K;
-  return 0;
-}
-
 extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
                                     const float* x_scale, int64_t ld_xs, const uint8_t* wq,
                                     const float* w_scale, const uint16_t* bias, int64_t N,
-                                    int32_t dtype, uint16_t* y, int64_t ldy, void* workspace,
-                                    size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
+                                    int32_t dtype, uint16_t* y, int64_t ldy, void* stream) {
   if (M < 0 || N < 1 || K < 1 || (dtype != TF_DTYPE_FP16 && dtype != TF_DTYPE_BF16))
     return TF_ERR_INVALID_ARG;
   if (K % 16 != 0) return TF_ERR_UNSUPPORTED;

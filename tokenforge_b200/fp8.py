@@ -10,7 +10,7 @@ Four operators, in the order a decoder layer runs them around its attention:
 
 The functions here are the direct launchers; :mod:`tokenforge_b200.ops` exports them and registers
 the same names as ``torch.ops.tokenforge.*`` with fakes for tracing. Calls enqueue on the current
-CUDA stream of the inputs' device; outputs and workspace come from PyTorch's caching allocator.
+CUDA stream of the inputs' device; outputs come from PyTorch's caching allocator.
 CPU tensors raise. The reference has no counterpart: it quantizes activations to e4m3
 (tokenforge/kernels/ops.py:130-156) but has no linear that consumes them.
 """
@@ -33,33 +33,41 @@ def _stream_dtype(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _on_gpu(device: torch.device, **tensors: torch.Tensor | None) -> None:
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{name} must be a CUDA tensor (tokenforge_b200 has no CPU path)")
-        if t.device != device:
-            raise ValueError(f"{name} is on {t.device}, expected {device}")
+def _gpu_index(t: torch.Tensor, name: str) -> int:
+    index = t.get_device()
+    if index < 0:
+        raise RuntimeError(f"{name} must be a CUDA tensor (tokenforge_b200 has no CPU path)")
+    return index
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """``t`` as 2-D rows with unit stride along the last dimension (a view where it can be)."""
+def _same_gpu(index: int, t: torch.Tensor, name: str) -> None:
+    if t.get_device() != index:
+        if _gpu_index(t, name) != index:
+            raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
+
+
+# The calls on few tokens take the host longer than the GPU, so the functions below look at every
+# tensor once and allocate with the cheapest calls (empty_like of a contiguous tensor, new_empty).
+
+
+def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """``t`` as 2-D rows with unit stride along the last dimension (a view where it can be), how
+    many rows, and their pitch. Rows that overlap (an expanded tensor) become a copy."""
     if t.dim() != 2:
         t = t.reshape(-1, t.shape[-1])
-    if t.stride(1) != 1 and t.shape[1] > 1:
-        t = t.contiguous()
-    return t
+    n, c = t.shape
+    pitch, step = t.stride()
+    if n <= 1:
+        pitch = c
+    if (step != 1 and c > 1) or pitch < c:
+        t, pitch = t.contiguous(), c
+    return t, n, pitch
 
 
-def _pitch(t: torch.Tensor) -> int:
-    """Row stride of 2-D rows; an expanded or overlapping one is refused by the caller's copy."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _no_overlap(t: torch.Tensor) -> torch.Tensor:
-    """Rows that overlap (an expanded tensor's stride of 0) as a copy with rows of their own."""
-    return t.contiguous() if t.shape[0] > 1 and t.stride(0) < t.shape[1] else t
+def _codes_like(x: torch.Tensor) -> torch.Tensor:
+    if x.is_contiguous():
+        return torch.empty_like(x, dtype=torch.float8_e4m3fn)
+    return x.new_empty(x.shape, dtype=torch.float8_e4m3fn)
 
 
 def _groups_of(columns: int, group_size: int) -> int:
@@ -96,24 +104,26 @@ def add_rmsnorm_fp8_quant(
         if residual.dtype != x.dtype:
             raise TypeError(f"residual must be {x.dtype} like x, got {residual.dtype}")
     groups = _groups_of(h, group_size)
-    dev = x.device
-    _on_gpu(dev, x=x, weight=weight, residual=residual)
-    lead = x.shape[:-1]
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((*lead, groups), dtype=torch.float32, device=dev)
-    total = x if residual is None else torch.empty(x.shape, dtype=x.dtype, device=dev)
-    x2 = _no_overlap(_rows(x))
-    t = x2.shape[0]
-    if t == 0:
-        return q, scale, total
-    r2 = None if residual is None else _no_overlap(_rows(residual))
+    index = _gpu_index(x, "x")
+    _same_gpu(index, weight, "weight")
+    q = _codes_like(x)
+    scale = x.new_empty((*x.shape[:-1], groups), dtype=torch.float32)
+    x2, t, ldx = _rows(x)
     if weight.stride(0) != 1:
         weight = weight.contiguous()
+    if residual is None:
+        total, rp, ldr, out = x, None, 0, None
+    else:
+        _same_gpu(index, residual, "residual")
+        total = torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+        r2, _, ldr = _rows(residual)
+        rp, out = r2.data_ptr(), total.data_ptr()
+    if t == 0:
+        return q, scale, total
     status = _lib.call_on(
-        dev, _lib.lib().tf_add_rmsnorm_fp8_quant,
-        x2.data_ptr(), t, h, _pitch(x2), None if r2 is None else r2.data_ptr(),
-        0 if r2 is None else _pitch(r2), weight.data_ptr(), eps, dtype, group_size,
-        q.data_ptr(), scale.data_ptr(), None if r2 is None else total.data_ptr(), h,
+        index, _lib.lib().tf_add_rmsnorm_fp8_quant,
+        x2.data_ptr(), t, h, ldx, rp, ldr, weight.data_ptr(), eps, dtype, group_size,
+        q.data_ptr(), scale.data_ptr(), out, h,
     )  # fmt: skip
     if status:
         _lib.check("tf_add_rmsnorm_fp8_quant", status)
@@ -133,18 +143,16 @@ def silu_mul_fp8_quant(
                          f"got {tuple(gate_up.shape)}")
     i = width // 2
     groups = _groups_of(i, group_size)
-    dev = gate_up.device
-    _on_gpu(dev, gate_up=gate_up)
+    index = _gpu_index(gate_up, "gate_up")
     lead = gate_up.shape[:-1]
-    q = torch.empty((*lead, i), dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((*lead, groups), dtype=torch.float32, device=dev)
-    g2 = _no_overlap(_rows(gate_up))
-    m = g2.shape[0]
+    q = gate_up.new_empty((*lead, i), dtype=torch.float8_e4m3fn)
+    scale = gate_up.new_empty((*lead, groups), dtype=torch.float32)
+    g2, m, ld = _rows(gate_up)
     if m == 0:
         return q, scale
     status = _lib.call_on(
-        dev, _lib.lib().tf_silu_mul_fp8_quant,
-        g2.data_ptr(), m, i, _pitch(g2), dtype, group_size, q.data_ptr(), scale.data_ptr(),
+        index, _lib.lib().tf_silu_mul_fp8_quant,
+        g2.data_ptr(), m, i, ld, dtype, group_size, q.data_ptr(), scale.data_ptr(),
     )  # fmt: skip
     if status:
         _lib.check("tf_silu_mul_fp8_quant", status)
@@ -159,17 +167,15 @@ def e4m3_quant_groups(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     c = x.shape[-1] if x.dim() else 0
     if c == 0:
         raise ValueError(f"x must be [..., C] with C >= 1, got {tuple(x.shape)}")
-    dev = x.device
-    _on_gpu(dev, x=x)
-    q = torch.empty(x.shape, dtype=torch.float8_e4m3fn, device=dev)
-    scale = torch.empty((*x.shape[:-1], -(-c // GROUP)), dtype=torch.float32, device=dev)
-    x2 = _no_overlap(_rows(x))
-    r = x2.shape[0]
+    index = _gpu_index(x, "x")
+    q = _codes_like(x)
+    scale = x.new_empty((*x.shape[:-1], -(-c // GROUP)), dtype=torch.float32)
+    x2, r, ldx = _rows(x)
     if r == 0:
         return q, scale
     status = _lib.call_on(
-        dev, _lib.lib().tf_e4m3_quant_groups,
-        x2.data_ptr(), r, c, _pitch(x2), dtype, q.data_ptr(), scale.data_ptr(),
+        index, _lib.lib().tf_e4m3_quant_groups,
+        x2.data_ptr(), r, c, ldx, dtype, q.data_ptr(), scale.data_ptr(),
     )  # fmt: skip
     if status:
         _lib.check("tf_e4m3_quant_groups", status)
@@ -220,28 +226,31 @@ def w8a8_block_linear(
             raise TypeError(f"bias must be {out_dtype} like the output, got {bias.dtype}")
         if bias.shape != (n,):
             raise ValueError(f"bias shape {tuple(bias.shape)} != {(n,)}")
-    dev = xq.device
-    _on_gpu(dev, xq=xq, x_scale=x_scale, wq=wq, w_scale=w_scale, bias=bias)
-    y = torch.empty((*lead, n), dtype=out_dtype, device=dev)
-    x2 = _rows(xq)
-    m = x2.shape[0]
+    index = _gpu_index(xq, "xq")
+    _same_gpu(index, x_scale, "x_scale")
+    _same_gpu(index, wq, "wq")
+    _same_gpu(index, w_scale, "w_scale")
+    bp = None
+    if bias is not None:
+        _same_gpu(index, bias, "bias")
+        if bias.stride(0) != 1:
+            bias = bias.contiguous()
+        bp = bias.data_ptr()
+    y = x_scale.new_empty((*lead, n), dtype=out_dtype)
+    x2, m, ldx = _rows(xq)
+    xp, wp = x2.data_ptr(), wq.data_ptr()
+    if xp % 16 or ldx % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+        xp, ldx = x2.data_ptr(), k
+    if wp % 16:
+        raise ValueError("wq must be 16-byte aligned")
     if m == 0:
         return y
-    if x2.data_ptr() % 16 or (m > 1 and (x2.stride(0) % 16 or x2.stride(0) < k)):
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    s2 = _no_overlap(_rows(x_scale))
-    if wq.data_ptr() % 16:
-        raise ValueError("wq must be 16-byte aligned")
-    if bias is not None and bias.stride(0) != 1:
-        bias = bias.contiguous()
+    s2, _, lds = _rows(x_scale)
     lib = _lib.lib()
-    ws_bytes = lib.tf_w8a8_workspace_bytes(m, n, k)
-    ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
     status = _lib.call_on(
-        dev, lib.tf_w8a8_block_linear,
-        x2.data_ptr(), m, k, _pitch(x2), s2.data_ptr(), _pitch(s2), wq.data_ptr(),
-        w_scale.data_ptr(), None if bias is None else bias.data_ptr(), n, dtype, y.data_ptr(), n,
-        None if ws is None else ws.data_ptr(), ws_bytes,
+        index, lib.tf_w8a8_block_linear,
+        xp, m, k, ldx, s2.data_ptr(), lds, wp, w_scale.data_ptr(), bp, n, dtype, y.data_ptr(), n,
     )  # fmt: skip
     if status:
         _lib.check("tf_w8a8_block_linear", status)
