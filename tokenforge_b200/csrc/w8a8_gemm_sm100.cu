@@ -130,9 +130,10 @@ __device__ __forceinline__ void set_max_regs_inc() {
   asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegs));
 }
 
+// The first 1024-byte boundary, as an offset from the array (an address rounded as an integer
+// would lose its address space, and every access become a generic one).
 __device__ __forceinline__ uint8_t* align_smem(uint8_t* raw) {
-  return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) &
-                                    ~static_cast<uintptr_t>(1023));
+  return raw + ((1024u - (smem_u32(raw) & 1023u)) & 1023u);
 }
 
 // K blocks [kb0, kb1) of share `index` of `splits`.
@@ -242,18 +243,38 @@ __device__ __forceinline__ void stage_row(uint8_t* out, int lane, V v) {
     *reinterpret_cast<uint4*>(out + staged(lane, 8 * c)) = o;
   }
 }
-// Copies the staged tokens m .. m + 31 to y, columns n .. n + cols: a lane a column, so rows of
-// any alignment are written in whole segments.
-template <typename T>
+// Copies the staged tokens m .. m + 31 to y, kCols columns from n on. Rows of 16-byte vectors: four
+// or more lanes a row. Others: a lane a column, four rows at a time, so that rows of any alignment
+// are written in whole segments.
+template <typename T, int kCols>
 __device__ __forceinline__ void copy_rows(const W8A8Args& a, const uint8_t* out, int64_t m,
-                                          int64_t n, int cols, int lane) {
+                                          int64_t n, bool vec, int lane) {
   const int rows = static_cast<int>(min(static_cast<int64_t>(32), a.M - m));
   T* y = reinterpret_cast<T*>(a.y) + m * a.ldy + n;
+  if (vec && n + kCols <= a.N) {
+    constexpr int kLanesPerRow = kCols / 8, kRowsPerStep = 32 / kLanesPerRow;
+    const int c = lane % kLanesPerRow * 8;
+#pragma unroll
+    for (int r = lane / kLanesPerRow; r < 32; r += kRowsPerStep)
+      if (r < rows)
+        *reinterpret_cast<uint4*>(y + r * a.ldy + c) =
+            *reinterpret_cast<const uint4*>(out + staged(r, c));
+    return;
+  }
 #pragma unroll 1
-  for (int r = 0; r < rows; ++r, y += a.ldy)
-#pragma unroll 1
-    for (int c = lane; c < cols && n + c < a.N; c += 32)
-      y[c] = *reinterpret_cast<const T*>(out + staged(r, c));
+  for (int r = 0; r < rows; r += 4) {
+    T v[4][kCols / 32];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < kCols / 32; ++k)
+        v[i][k] = *reinterpret_cast<const T*>(out + staged(r + i, lane + 32 * k));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < kCols / 32; ++k)
+        if (r + i < rows && n + lane + 32 * k < a.N) y[(r + i) * a.ldy + lane + 32 * k] = v[i][k];
+  }
 }
 // Lane l's bias of column n + l (0 past N).
 template <typename T>
@@ -269,12 +290,9 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                : "memory");
   asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-// The stores issued by this thread have read their shared memory / are complete.
+// The stores issued by this thread have read their shared memory.
 __device__ __forceinline__ void tma_store_read_wait() {
   asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
-}
-__device__ __forceinline__ void tma_store_wait() {
-  asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
 }
 
 template <typename T>
@@ -532,18 +550,19 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
                            static_cast<int>(m));
       } else {
         __syncwarp();
-        copy_rows<T>(p.a, out, m - lane, n0 + c0, C::kColsPerThread, lane);
+        copy_rows<T, C::kColsPerThread>(p.a, out, m - lane, n0 + c0, false, lane);
         __syncwarp();
       }
     }
   }
-  if (lane == 0) tma_store_wait();
+  if (lane == 0) tma_store_read_wait();
   __syncwarp();
 
   if (p.splits > 1) {
     // Partial tiles as [column][lane] in the (drained) stages. Units of 32 columns are dealt to
-    // the shares, and a share's to its two warps of a quadrant, which sum them over the shares
-    // in order.
+    // the shares, and a share's to its two warps of a quadrant, which sum them over the shares in
+    // an order of the unit's own (its owner's share first, so that the CTAs do not all read the
+    // same one at a time).
     float* part = reinterpret_cast<float*>(smem);
 #pragma unroll
     for (int i = 0; i < N2; ++i) {
@@ -559,9 +578,13 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
       for (int e = 0; e < 32; ++e) v[e] = 0.f;
 #pragma unroll 1
       for (int k = 0; k < p.splits; ++k) {
-        const uint32_t at = map_to_rank(smem_u32(part + 32 * unit * kLanes + row), 2 * k + side);
+        const int from = share + k < p.splits ? share + k : share + k - p.splits;
+        const uint32_t at = map_to_rank(smem_u32(part + 32 * unit * kLanes + row), 2 * from + side);
+        float w[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] += ld_cluster(at + 4 * e * kLanes);
+        for (int e = 0; e < 32; ++e) w[e] = ld_cluster(at + 4 * e * kLanes);
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] += w[e];
       }
       if (p.a.bias != nullptr) {
         const float mine = bias_of<T>(p.a, n0 + 32 * unit + lane);
@@ -570,7 +593,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
       }
       stage_row<T, 32>(out, lane, [&](int i) { return v[i]; });
       __syncwarp();
-      copy_rows<T>(p.a, out, m - lane, n0 + 32 * unit, 32, lane);
+      copy_rows<T, 32>(p.a, out, m - lane, n0 + 32 * unit, p.tma_out != 0, lane);
       __syncwarp();
     }
   }
