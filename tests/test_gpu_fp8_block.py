@@ -294,6 +294,27 @@ def test_quant_every_value(dtype: torch.dtype, device: torch.device) -> None:
     assert torch.equal(q.cpu().view(torch.uint8), codes.view(torch.uint8))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_quant_every_value_under_every_maximum(dtype: torch.dtype, device: torch.device) -> None:
+    """Each positive finite 16-bit value as a group's maximum over every value up to it, against
+    the GPU's IEEE division (torch's tensor by tensor division): what the kernel's single
+    residual correction rests on."""
+    v = torch.arange(65536, dtype=torch.int32).to(torch.uint16).view(dtype).to(device)
+    v = v[torch.isfinite(v)]
+    body = torch.cat([v, v.new_zeros(-len(v) % 127)]).view(1, -1, 127)
+    tops = v[v > 0]
+    for i in range(0, len(tops), 128):
+        t = tops[i : i + 128].view(-1, 1, 1)
+        x = torch.cat([torch.where(body.abs() <= t, body, torch.zeros_like(body)),
+                       t.expand(-1, body.shape[1], 1)], 2).reshape(-1, 128)
+        q, s = ops.e4m3_quant_groups(x)
+        amax = x.float().abs().amax(1, keepdim=True)
+        want = torch.div(amax, torch.full_like(amax, 448.0)).clamp(min=FP8_MIN_SCALE)
+        assert torch.equal(s, want)
+        codes = torch.div(x.float(), want.expand(-1, 128)).clamp(-448, 448).to(E4M3)
+        assert torch.equal(q.view(torch.uint8), codes.view(torch.uint8)), f"maxima from {i}"
+
+
 @pytest.mark.parametrize("c", [256, 250])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_special_values(c: int, dtype: torch.dtype, device: torch.device) -> None:

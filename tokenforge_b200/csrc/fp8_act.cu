@@ -60,6 +60,16 @@ __device__ __forceinline__ float rstd_f(float sumsq, int64_t H, float eps) {
   return __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(sumsq, static_cast<float>(H)), eps)));
 }
 
+// y = h * rstd * weight of one vector.
+template <typename T>
+__device__ __forceinline__ void norm8(const uint4& h, const uint4& w, float rstd, float (&y)[8]) {
+  float gw[8];
+  widen8<T>(h, y);
+  widen8<T>(w, gw);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) y[e] = y[e] * rstd * gw[e];
+}
+
 // ------------------------------------------------------------------ residual + RMSNorm + FP8
 
 struct NormArgs {
@@ -74,93 +84,178 @@ struct NormArgs {
   int group;  // 128, or 0 for one scale per row
 };
 
-// One CTA per row, VPT 16-byte vectors per thread, the row's sum held in registers.
+// CTAs walk the rows (row, row + grid, ...), VPT 16-byte vectors of a row per thread, the row's sum
+// held in registers. A row's loads, its two reductions and its stores follow each other, so the
+// next row's loads are issued before the current one is reduced: with a CTA per row and no
+// lookahead, 8192 rows of 3584 bf16 took 40.4 us.
+// Resident CTAs of 512 threads an SM, by registers (smaller CTAs in proportion).
+constexpr int norm_ctas(int vpt) { return vpt <= 2 ? 2 : 1; }
+
 template <typename T, int VPT>
-__global__ void __launch_bounds__(512) add_rmsnorm_row_kernel(const NormArgs a) {
-  __shared__ float sh_sum[32];
-  __shared__ uint32_t sh_max[32];
-  const int64_t row = blockIdx.x;
+__global__ void __launch_bounds__(512, norm_ctas(VPT)) add_rmsnorm_row_kernel(const NormArgs a) {
+  constexpr bool kAhead = VPT <= 4;  // eight vectors and the next eight do not fit the registers
+  __shared__ float sh_sum[2][32];
+  __shared__ uint32_t sh_max[2][32];
   const int tid = threadIdx.x, nt = blockDim.x;
   const int nvec = static_cast<int>(a.H / 8);
+  const int groups = (nvec + kGroupVecs - 1) / kGroupVecs;
   const uint4* w = reinterpret_cast<const uint4*>(a.weight);
-  const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
-  const uint4* rr = reinterpret_cast<const uint4*>(a.residual + row * a.ldr);
-  uint4* sr = reinterpret_cast<uint4*>(a.sum_out + row * a.ldo);
-  uint4 g[VPT], v[VPT];
+  uint4 g[VPT], x[VPT], r[VPT];
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int j = tid + nt * i;
     g[i] = j < nvec ? __ldg(w + j) : make_uint4(0, 0, 0, 0);
   }
+  auto load = [&](int64_t row) {
+    const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
+    const uint4* rr = reinterpret_cast<const uint4*>(a.residual + row * a.ldr);
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      const int j = tid + nt * i;
+      x[i] = j < nvec ? xr[j] : make_uint4(0, 0, 0, 0);
+      if (a.residual != nullptr) r[i] = j < nvec ? rr[j] : make_uint4(0, 0, 0, 0);
+    }
+  };
   // x and the residual (and the outputs) may belong to the preceding kernel on the stream.
   pdl_wait();
+  if (kAhead) load(blockIdx.x);
+  int phase = 0;
+  for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, phase ^= 1) {
+    if (!kAhead) load(row);
+    uint4 v[VPT];
+    if (a.residual != nullptr) {
+      uint4* sr = reinterpret_cast<uint4*>(a.sum_out + row * a.ldo);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    const int j = tid + nt * i;
-    v[i] = j < nvec ? xr[j] : make_uint4(0, 0, 0, 0);
+      for (int i = 0; i < VPT; ++i) {
+        float fx[8], fr[8];
+        widen8<T>(x[i], fx);
+        widen8<T>(r[i], fr);
+        uint32_t* o = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          o[e] = narrow2(fx[2 * e] + fr[2 * e], fx[2 * e + 1] + fr[2 * e + 1], T());
+        if (tid + nt * i < nvec) sr[tid + nt * i] = v[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) v[i] = x[i];
+    }
+    if (kAhead && row + gridDim.x < a.T) load(row + gridDim.x);
+    float sumsq = 0.f;
+#pragma unroll
+    for (int i = 0; i < VPT; ++i) {
+      float f[8];
+      widen8<T>(v[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sumsq = fmaf(f[e], f[e], sumsq);
+    }
+    const float rstd = rstd_f(block_sum_f(sumsq, sh_sum[phase]), a.H, a.eps);
+    uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.H);
+    // 0 * rstd may be NaN past the row: those lanes take no part in the maxima.
+    if (a.group != 0) {
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        const int j = tid + nt * i;
+        float y[8];
+        norm8<T>(v[i], g[i], rstd, y);
+        const float s = scale_of_bits(half_warp_max(j < nvec ? max_bits8(y) : 0u));
+        if (j < nvec) {
+          if (j % kGroupVecs == 0) a.scale[row * groups + j / kGroupVecs] = s;
+          qr[j] = codes8<false>(y, s);
+        }
+      }
+    } else {
+      uint32_t m = 0;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float y[8];
+        norm8<T>(v[i], g[i], rstd, y);
+        if (tid + nt * i < nvec) m = max(m, max_bits8(y));
+      }
+      const float s = scale_of_bits(block_max_bits(m, sh_max[phase]));
+      if (tid == 0) a.scale[row] = s;
+#pragma unroll
+      for (int i = 0; i < VPT; ++i) {
+        float y[8];
+        norm8<T>(v[i], g[i], rstd, y);  // the same operations: the same bits
+        if (tid + nt * i < nvec) qr[tid + nt * i] = codes8<false>(y, s);
+      }
+    }
   }
+}
+
+// Rows that are not 16-byte vectors, up to 8192 columns: a CTA per row, a warp per 128-column
+// group (GP groups a warp), lane l of it columns l, l + 32, l + 64, l + 96, in registers.
+template <typename T, int GP>
+__global__ void __launch_bounds__(512) add_rmsnorm_group_kernel(const NormArgs a) {
+  __shared__ float sh_sum[32];
+  __shared__ uint32_t sh_max[32];
+  const int64_t row = blockIdx.x;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  const int H = static_cast<int>(a.H), groups = (H + kGroup - 1) / kGroup;
+  const T* w = reinterpret_cast<const T*>(a.weight);
+  const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
+  const T* rr = reinterpret_cast<const T*>(a.residual) + row * a.ldr;
+  T* sr = reinterpret_cast<T*>(a.sum_out) + row * a.ldo;
+  auto column = [&](int p, int j) { return (warp + nw * p) * kGroup + lane + 32 * j; };
+  float g[GP][4], y[GP][4];
+#pragma unroll
+  for (int p = 0; p < GP; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) g[p][j] = column(p, j) < H ? widen(w[column(p, j)]) : 0.f;
+  pdl_wait();
+#pragma unroll
+  for (int p = 0; p < GP; ++p)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[p][j] = column(p, j) < H ? widen(xr[column(p, j)]) : 0.f;
   if (a.residual != nullptr) {
-    uint4 r[VPT];
+    float r[GP][4];
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = tid + nt * i;
-      r[i] = j < nvec ? rr[j] : make_uint4(0, 0, 0, 0);
-    }
+    for (int p = 0; p < GP; ++p)
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = tid + nt * i;
-      float fx[8], fr[8];
-      widen8<T>(v[i], fx);
-      widen8<T>(r[i], fr);
-      uint32_t* o = reinterpret_cast<uint32_t*>(&v[i]);
+      for (int j = 0; j < 4; ++j) r[p][j] = column(p, j) < H ? widen(rr[column(p, j)]) : 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        o[e] = narrow2(fx[2 * e] + fr[2 * e], fx[2 * e + 1] + fr[2 * e + 1], T());
-      if (j < nvec) sr[j] = v[i];
-    }
+    for (int p = 0; p < GP; ++p)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        T t;
+        narrow(y[p][j] + r[p][j], &t);
+        if (column(p, j) < H) sr[column(p, j)] = t;
+        y[p][j] = widen(t);
+      }
   }
   float sumsq = 0.f;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    float f[8];
-    widen8<T>(v[i], f);
+  for (int p = 0; p < GP; ++p)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) sumsq = fmaf(f[e], f[e], sumsq);
-  }
+    for (int j = 0; j < 4; ++j) sumsq = fmaf(y[p][j], y[p][j], sumsq);
   const float rstd = rstd_f(block_sum_f(sumsq, sh_sum), a.H, a.eps);
-  float y[VPT][8];
-  uint32_t m[VPT];
+  uint32_t m[GP], all = 0;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i) {
-    float gw[8];
-    widen8<T>(v[i], y[i]);
-    widen8<T>(g[i], gw);
+  for (int p = 0; p < GP; ++p) {
+    m[p] = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[i][e] = y[i][e] * rstd * gw[e];
-    m[i] = tid + nt * i < nvec ? max_bits8(y[i]) : 0u;  // 0 * rstd may be NaN past the row
-  }
-  uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.H);
-  if (a.group != 0) {
-    const int groups = (nvec + kGroupVecs - 1) / kGroupVecs;
-#pragma unroll
-    for (int i = 0; i < VPT; ++i) {
-      const int j = tid + nt * i;
-      const float s = scale_of_bits(half_warp_max(m[i]));
-      if (j < nvec) {
-        if (j % kGroupVecs == 0) a.scale[row * groups + j / kGroupVecs] = s;
-        qr[j] = codes8<false>(y[i], group_div(s));
-      }
+    for (int j = 0; j < 4; ++j) {
+      y[p][j] = y[p][j] * rstd * g[p][j];
+      if (column(p, j) < H) m[p] = max(m[p], abs_bits(y[p][j]));
     }
-  } else {
-    uint32_t mm = 0;
+    all = max(all, m[p]);
+  }
+  float s = 0.f;
+  if (a.group == 0) {
+    s = scale_of_bits(block_max_bits(all, sh_max));
+    if (threadIdx.x == 0) a.scale[row] = s;
+  }
+  uint8_t* qr = a.q + row * a.H;
 #pragma unroll
-    for (int i = 0; i < VPT; ++i) mm = max(mm, m[i]);
-    const float s = scale_of_bits(block_max_bits(mm, sh_max));
-    if (tid == 0) a.scale[row] = s;
-    const GroupDiv d = group_div(s);
+  for (int p = 0; p < GP; ++p) {
+    if (a.group != 0) {
+      s = scale_of_bits(warp_max_bits(m[p]));
+      if (lane == 0 && warp + nw * p < groups) a.scale[row * groups + warp + nw * p] = s;
+    }
 #pragma unroll
-    for (int i = 0; i < VPT; ++i)
-      if (tid + nt * i < nvec) qr[tid + nt * i] = codes8<false>(y[i], d);
+    for (int j = 0; j < 4; ++j)
+      if (column(p, j) < H) qr[column(p, j)] = code1<false>(y[p][j], s);
   }
 }
 
@@ -192,9 +287,7 @@ __global__ void __launch_bounds__(512) add_rmsnorm_any_kernel(const NormArgs a) 
   const T* hr = a.residual != nullptr ? sr : xr;
   auto y_of = [&](int64_t c) { return widen(hr[c]) * rstd * widen(w[c]); };
   uint8_t* qr = a.q + row * a.H;
-  auto put = [&](int64_t c, const GroupDiv& d) {
-    qr[c] = static_cast<uint8_t>(cvt_e4m3x2(divide<false>(y_of(c), d), 0.f) & 0xFFu);
-  };
+  auto put = [&](int64_t c, float s) { qr[c] = code1<false>(y_of(c), s); };
   if (a.group != 0) {
     const int lane = threadIdx.x & 31;
     const int64_t groups = (a.H + kGroup - 1) / kGroup;
@@ -204,16 +297,14 @@ __global__ void __launch_bounds__(512) add_rmsnorm_any_kernel(const NormArgs a) 
       for (int64_t c = g * kGroup + lane; c < c1; c += 32) m = max(m, abs_bits(y_of(c)));
       const float s = scale_of_bits(warp_max_bits(m));
       if (lane == 0) a.scale[row * groups + g] = s;
-      const GroupDiv d = group_div(s);
-      for (int64_t c = g * kGroup + lane; c < c1; c += 32) put(c, d);
+      for (int64_t c = g * kGroup + lane; c < c1; c += 32) put(c, s);
     }
   } else {
     uint32_t m = 0;
     for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) m = max(m, abs_bits(y_of(c)));
     const float s = scale_of_bits(block_max_bits(m, sh_max));
     if (threadIdx.x == 0) a.scale[row] = s;
-    const GroupDiv d = group_div(s);
-    for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) put(c, d);
+    for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) put(c, s);
   }
 }
 
@@ -233,12 +324,14 @@ struct SiluSource {
   static __device__ __forceinline__ Raw load(const T* row, int64_t j, int64_t C) {
     return Raw{ldg_stream_v4(row + 8 * j), ldg_stream_v4(row + C + 8 * j)};
   }
-  static __device__ __forceinline__ void value(const Raw& r, float (&y)[8]) {
+  // y, and the bits of its largest magnitude.
+  static __device__ __forceinline__ uint32_t value(const Raw& r, float (&y)[8]) {
     float g[8], u[8];
     widen8<T>(r.g, g);
     widen8<T>(r.u, u);
 #pragma unroll
     for (int e = 0; e < 8; ++e) y[e] = __fdividef(g[e], 1.0f + __expf(-g[e])) * u[e];
+    return max_bits8(y);
   }
 };
 template <typename T>
@@ -253,8 +346,14 @@ struct CopySource {
   static __device__ __forceinline__ Raw load(const T* row, int64_t j, int64_t) {
     return Raw{ldg_stream_v4(row + 8 * j)};
   }
-  static __device__ __forceinline__ void value(const Raw& r, float (&y)[8]) {
+  // The maximum of the 16-bit patterns, two at a time: the same order as the widened values'.
+  static __device__ __forceinline__ uint32_t value(const Raw& r, float (&y)[8]) {
     widen8<T>(r.x, y);
+    constexpr uint32_t kAbs = 0x7FFF7FFFu;
+    const uint32_t m = __vmaxu2(__vmaxu2(r.x.x & kAbs, r.x.y & kAbs),
+                                __vmaxu2(r.x.z & kAbs, r.x.w & kAbs));
+    const uint32_t top = max(m & 0xFFFFu, m >> 16);
+    return __float_as_uint(widen2(top, T()).x);
   }
 };
 
@@ -266,51 +365,51 @@ struct GroupArgs {
 };
 
 // Scale per group, aligned rows. Row r's C / 8 vectors are padded to whole groups of 16; the
-// padded vectors of all rows, in order, are dealt to half warps, U of them a thread.
+// padded vectors of all rows, in order, are dealt to half warps, U of them a thread, so that U
+// (or 2 U) loads are in flight before the first one is used.
 template <typename T, template <typename> class Source, int U>
-__global__ void __launch_bounds__(256) quant_groups_kernel(const GroupArgs a) {
-  const int64_t nvec = a.C / 8;
-  const int64_t groups = (nvec + kGroupVecs - 1) / kGroupVecs;
-  const int64_t total = a.R * groups * kGroupVecs;
+__global__ void __launch_bounds__(256) quant_groups_kernel(const GroupArgs a, const FastDiv per_row) {
+  const int nvec = static_cast<int>(a.C / 8);
+  const int groups = static_cast<int>(per_row.d) / kGroupVecs;
+  const uint32_t total = static_cast<uint32_t>(a.R) * per_row.d;
   const T* x = reinterpret_cast<const T*>(a.x);
   pdl_wait();
-  const int64_t base = static_cast<int64_t>(blockIdx.x) * (256 * U) + threadIdx.x;
+  const uint32_t base = blockIdx.x * (256 * U) + threadIdx.x;
   typename Source<T>::Raw raw[U];
-  int64_t row[U], vec[U];
 #pragma unroll
   for (int i = 0; i < U; ++i) {
-    const int64_t s = base + 256 * i;
-    row[i] = s / (groups * kGroupVecs);
-    vec[i] = s - row[i] * (groups * kGroupVecs);
-    if (s >= total) vec[i] = nvec;
-    if (vec[i] < nvec) raw[i] = Source<T>::load(x + row[i] * a.ldx, vec[i], a.C);
+    const uint32_t s = base + 256 * i;
+    const uint32_t row = div_by(s, per_row);
+    const int vec = static_cast<int>(s - row * per_row.d);
+    if (s < total && vec < nvec)
+      raw[i] = Source<T>::load(x + static_cast<int64_t>(row) * a.ldx, vec, a.C);
   }
 #pragma unroll
   for (int i = 0; i < U; ++i) {
+    const uint32_t s = base + 256 * i;
+    const uint32_t row = div_by(s, per_row);
+    const int vec = static_cast<int>(s - row * per_row.d);
+    const bool ok = s < total && vec < nvec;
     float y[8];
-    uint32_t m = 0;
-    if (vec[i] < nvec) {
-      Source<T>::value(raw[i], y);
-      m = max_bits8(y);
-    }
-    const float s = scale_of_bits(half_warp_max(m));
-    if (vec[i] < nvec) {
-      if (vec[i] % kGroupVecs == 0) a.scale[row[i] * groups + vec[i] / kGroupVecs] = s;
-      reinterpret_cast<uint2*>(a.q + row[i] * a.C)[vec[i]] =
-          codes8<Source<T>::kExact>(y, group_div(s));
+    const uint32_t m = Source<T>::value(raw[i], y);
+    const float sc = scale_of_bits(half_warp_max(ok ? m : 0u));
+    if (ok) {
+      if (vec % kGroupVecs == 0) a.scale[static_cast<int64_t>(row) * groups + vec / kGroupVecs] = sc;
+      reinterpret_cast<uint2*>(a.q + row * a.C)[vec] = codes8<Source<T>::kExact>(y, sc);
     }
   }
 }
 
 // Scale per group, any C and alignment: a warp per group, columns lane, lane + 32, ...
 template <typename T, template <typename> class Source>
-__global__ void __launch_bounds__(256) quant_groups_any_kernel(const GroupArgs a) {
-  const int64_t groups = (a.C + kGroup - 1) / kGroup;
-  const int64_t id = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(256) quant_groups_any_kernel(const GroupArgs a,
+                                                              const FastDiv per_row) {
+  const uint32_t groups = per_row.d;
+  const uint32_t id = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
   pdl_wait();
-  if (id >= a.R * groups) return;
-  const int64_t row = id / groups, g = id - row * groups;
+  if (id >= static_cast<uint32_t>(a.R) * groups) return;
+  const int64_t row = div_by(id, per_row), g = id - static_cast<uint32_t>(row) * groups;
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
   float y[4];
   uint32_t m = 0;
@@ -322,43 +421,43 @@ __global__ void __launch_bounds__(256) quant_groups_any_kernel(const GroupArgs a
   }
   const float s = scale_of_bits(warp_max_bits(m));
   if (lane == 0) a.scale[id] = s;
-  const GroupDiv d = group_div(s);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int64_t c = g * kGroup + lane + 32 * i;
-    if (c < a.C)
-      a.q[row * a.C + c] =
-          static_cast<uint8_t>(cvt_e4m3x2(divide<Source<T>::kExact>(y[i], d), 0.f) & 0xFFu);
+    if (c < a.C) a.q[row * a.C + c] = code1<Source<T>::kExact>(y[i], s);
   }
 }
 
-// One scale per row, aligned rows of at most 1024 * VPT vectors: a CTA per row, y in registers.
+// One scale per row, aligned rows of at most 1024 * VPT vectors: a CTA walks the rows, y in
+// registers, the next row's loads issued before the current row's maximum is reduced.
 template <typename T, template <typename> class Source, int VPT>
 __global__ void __launch_bounds__(1024) quant_row_kernel(const GroupArgs a) {
-  __shared__ uint32_t sh_max[32];
-  const int64_t row = blockIdx.x;
+  __shared__ uint32_t sh_max[2][32];
   const int nvec = static_cast<int>(a.C / 8), tid = threadIdx.x, nt = blockDim.x;
-  const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
   pdl_wait();
   typename Source<T>::Raw raw[VPT];
+  auto load = [&](int64_t row) {
+    const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (tid + nt * i < nvec) raw[i] = Source<T>::load(xr, tid + nt * i, a.C);
-  float y[VPT][8];
-  uint32_t m = 0;
+    for (int i = 0; i < VPT; ++i)
+      if (tid + nt * i < nvec) raw[i] = Source<T>::load(xr, tid + nt * i, a.C);
+  };
+  load(blockIdx.x);
+  int phase = 0;
+  for (int64_t row = blockIdx.x; row < a.R; row += gridDim.x, phase ^= 1) {
+    float y[VPT][8];
+    uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (tid + nt * i < nvec) {
-      Source<T>::value(raw[i], y[i]);
-      m = max(m, max_bits8(y[i]));
-    }
-  const float s = scale_of_bits(block_max_bits(m, sh_max));
-  if (tid == 0) a.scale[row] = s;
-  const GroupDiv d = group_div(s);
-  uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.C);
+    for (int i = 0; i < VPT; ++i)
+      if (tid + nt * i < nvec) m = max(m, Source<T>::value(raw[i], y[i]));
+    if (row + gridDim.x < a.R) load(row + gridDim.x);
+    const float s = scale_of_bits(block_max_bits(m, sh_max[phase]));
+    if (tid == 0) a.scale[row] = s;
+    uint2* qr = reinterpret_cast<uint2*>(a.q + row * a.C);
 #pragma unroll
-  for (int i = 0; i < VPT; ++i)
-    if (tid + nt * i < nvec) qr[tid + nt * i] = codes8<Source<T>::kExact>(y[i], d);
+    for (int i = 0; i < VPT; ++i)
+      if (tid + nt * i < nvec) qr[tid + nt * i] = codes8<Source<T>::kExact>(y[i], s);
+  }
 }
 
 // One scale per row, any C and alignment: two sweeps (the second hits L2).
@@ -373,16 +472,14 @@ __global__ void __launch_bounds__(1024) quant_row_any_kernel(const GroupArgs a) 
     m = max(m, abs_bits(Source<T>::one(xr, c, a.C)));
   const float s = scale_of_bits(block_max_bits(m, sh_max));
   if (threadIdx.x == 0) a.scale[row] = s;
-  const GroupDiv d = group_div(s);
   for (int64_t c = threadIdx.x; c < a.C; c += blockDim.x)
-    a.q[row * a.C + c] = static_cast<uint8_t>(
-        cvt_e4m3x2(divide<Source<T>::kExact>(Source<T>::one(xr, c, a.C), d), 0.f) & 0xFFu);
+    a.q[row * a.C + c] = code1<Source<T>::kExact>(Source<T>::one(xr, c, a.C), s);
 }
 
 // ----------------------------------------------------------------------------- host side
 
-template <typename Args>
-int launch(void (*kernel)(Args), int64_t grid, int threads, cudaStream_t stream, const Args& a) {
+template <typename... Args>
+int launch(void (*kernel)(Args...), int64_t grid, int threads, cudaStream_t stream, Args... a) {
   if (grid > 0x7fffffffLL) return TF_ERR_TOO_LARGE;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(grid));
@@ -393,7 +490,7 @@ int launch(void (*kernel)(Args), int64_t grid, int threads, cudaStream_t stream,
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
   cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a...);
   if (e != cudaSuccess) {
     last_cuda_error() = static_cast<int>(e);
     return TF_ERR_CUDA;
@@ -409,15 +506,28 @@ int launch_norm(const NormArgs& a, cudaStream_t stream) {
                    aligned16(a.weight) && (reinterpret_cast<uintptr_t>(a.q) & 7u) == 0 &&
                    (a.residual == nullptr || (aligned16(a.residual) && a.ldr % 8 == 0 &&
                                               aligned16(a.sum_out) && a.ldo % 8 == 0));
+  if (!vec && a.H <= 64 * kGroup) {
+    const int groups = static_cast<int>(cdiv(a.H, kGroup));
+    const int gp = groups <= 16 ? 1 : groups <= 32 ? 2 : 4;
+    const int threads = 32 * static_cast<int>(cdiv(groups, gp));
+    switch (gp) {
+      case 1: return launch(add_rmsnorm_group_kernel<T, 1>, a.T, threads, stream, a);
+      case 2: return launch(add_rmsnorm_group_kernel<T, 2>, a.T, threads, stream, a);
+      default: return launch(add_rmsnorm_group_kernel<T, 4>, a.T, threads, stream, a);
+    }
+  }
   if (!vec) return launch(add_rmsnorm_any_kernel<T>, a.T, 512, stream, a);
   const int64_t nvec = a.H / 8;
-  const int vpt = nvec <= 512 ? 1 : nvec <= 1024 ? 2 : nvec <= 2048 ? 4 : 8;
+  // Two vectors a thread from 64 of them on: half the threads a row, so twice the rows in flight
+  // (3584 columns, 8192 rows: 34.0 us, 39.0 with one vector).
+  const int vpt = nvec <= 64 ? 1 : nvec <= 1024 ? 2 : nvec <= 2048 ? 4 : 8;
   const int threads = static_cast<int>(cdiv(cdiv(nvec, vpt), 32) * 32);
+  const int64_t grid = std::min<int64_t>(a.T, 148 * (512 * norm_ctas(vpt) / threads));
   switch (vpt) {
-    case 1: return launch(add_rmsnorm_row_kernel<T, 1>, a.T, threads, stream, a);
-    case 2: return launch(add_rmsnorm_row_kernel<T, 2>, a.T, threads, stream, a);
-    case 4: return launch(add_rmsnorm_row_kernel<T, 4>, a.T, threads, stream, a);
-    default: return launch(add_rmsnorm_row_kernel<T, 8>, a.T, threads, stream, a);
+    case 1: return launch(add_rmsnorm_row_kernel<T, 1>, grid, threads, stream, a);
+    case 2: return launch(add_rmsnorm_row_kernel<T, 2>, grid, threads, stream, a);
+    case 4: return launch(add_rmsnorm_row_kernel<T, 4>, grid, threads, stream, a);
+    default: return launch(add_rmsnorm_row_kernel<T, 8>, grid, threads, stream, a);
   }
 }
 
@@ -428,12 +538,28 @@ bool vec_rows(const GroupArgs& a) {
 
 template <typename T, template <typename> class Source>
 int launch_groups(const GroupArgs& a, cudaStream_t stream) {
-  const int64_t groups = cdiv(a.C, kGroup);
-  if (!vec_rows(a))
-    return launch(quant_groups_any_kernel<T, Source>, cdiv(a.R * groups, 8), 256, stream, a);
   constexpr int U = 4;
-  return launch(quant_groups_kernel<T, Source, U>, cdiv(a.R * groups * kGroupVecs, 256 * U), 256,
-                stream, a);
+  const bool vec = vec_rows(a);
+  const int64_t groups = cdiv(a.C, kGroup);
+  const int64_t per_row = vec ? groups * kGroupVecs : groups;  // slots, of vectors or of groups
+  if (per_row >= (int64_t(1) << 30)) return TF_ERR_TOO_LARGE;
+  const FastDiv div = fast_div(static_cast<uint32_t>(per_row));
+  // Slots are 31-bit numbers: more rows than that take several launches.
+  const int64_t most = ((int64_t(1) << 31) - 256 * U - 1) / per_row;
+  for (int64_t r0 = 0; r0 < a.R; r0 += most) {
+    GroupArgs part = a;
+    part.R = std::min(most, a.R - r0);
+    part.x = a.x + r0 * a.ldx;
+    part.q = a.q + r0 * a.C;
+    part.scale = a.scale + r0 * groups;
+    const int64_t slots = part.R * per_row;
+    const int st = vec ? launch(quant_groups_kernel<T, Source, U>, cdiv(slots, 256 * U), 256,
+                                stream, part, div)
+                       : launch(quant_groups_any_kernel<T, Source>, cdiv(slots, 8), 256, stream,
+                                part, div);
+    if (st != TF_OK) return st;
+  }
+  return TF_OK;
 }
 
 template <typename T, template <typename> class Source>
@@ -443,11 +569,12 @@ int launch_rows(const GroupArgs& a, cudaStream_t stream) {
     return launch(quant_row_any_kernel<T, Source>, a.R, 1024, stream, a);
   const int vpt = nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : nvec <= 3072 ? 3 : 4;
   const int threads = static_cast<int>(cdiv(cdiv(nvec, vpt), 32) * 32);
+  const int64_t grid = std::min<int64_t>(a.R, 148 * (1024 / threads));
   switch (vpt) {
-    case 1: return launch(quant_row_kernel<T, Source, 1>, a.R, threads, stream, a);
-    case 2: return launch(quant_row_kernel<T, Source, 2>, a.R, threads, stream, a);
-    case 3: return launch(quant_row_kernel<T, Source, 3>, a.R, threads, stream, a);
-    default: return launch(quant_row_kernel<T, Source, 4>, a.R, threads, stream, a);
+    case 1: return launch(quant_row_kernel<T, Source, 1>, grid, threads, stream, a);
+    case 2: return launch(quant_row_kernel<T, Source, 2>, grid, threads, stream, a);
+    case 3: return launch(quant_row_kernel<T, Source, 3>, grid, threads, stream, a);
+    default: return launch(quant_row_kernel<T, Source, 4>, grid, threads, stream, a);
   }
 }
 

@@ -47,10 +47,15 @@ __device__ __forceinline__ void widen8(const uint4& v, float (&f)[8]) {
 // its maximum, its scale and (below) every code of it, as in the elementary operations.
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
 
-// scale = max(amax / 448, 1 / (448 * 512)); a NaN maximum gives a NaN scale.
+// scale = max(amax / 448, 1 / (448 * 512)) with the IEEE quotient: q0 = amax * RN(1 / 448) is
+// within one ulp of it, and one residual correction rounds it correctly (tf_rmsnorm.cuh names the
+// method), where the result is above the floor (far above the subnormal range). Inf and NaN have
+// no residual: they keep q0.
 __device__ __forceinline__ float scale_of_bits(uint32_t amax_bits) {
+  constexpr float kInv = 1.0f / kFp8Max;
   const float a = __uint_as_float(amax_bits);
-  const float s = __fdiv_rn(a, kFp8Max);
+  float s = __fmul_rn(a, kInv);
+  if (amax_bits < 0x7F800000u) s = __fmaf_rn(__fmaf_rn(-s, kFp8Max, a), kInv, s);
   return s < kMinScale ? kMinScale : s;
 }
 
@@ -61,39 +66,55 @@ __device__ __forceinline__ uint32_t half_warp_max(uint32_t v) {
   return v;
 }
 
-// Divisor of one group. kExact: the quotient y / scale is the IEEE division's (two residual
-// corrections of y * RN(1 / scale), tf_rmsnorm.cuh names the method): used where y is an input
-// value, so that the codes are the exact ones. Otherwise y * RN(1 / scale): y carries a few
-// fp32 roundings of its own already, and 1.5 more of 2^-24 are far below e4m3's half step 2^-4.
-// Every quotient whose code is not zero has |y| >= 2^-28 (scale >= 2^-17.8), so no step below
-// leaves the normal range where it counts; scales reach 7.6e35 (bf16), whose reciprocal is
-// normal.
-struct GroupDiv {
-  float b, r;
-};
-__device__ __forceinline__ GroupDiv group_div(float scale) {
-  return GroupDiv{scale, __frcp_rn(scale)};
-}
+// e4m3 codes of eight values under one scale. kExact: each quotient is the IEEE division's (one
+// residual correction of y * RN(1 / scale)); used where y is an input value of 16 bits, so that
+// the codes are the exact ones. One correction is within 2^-22 ulp of the quotient's rounding; it
+// could only change a code where a quotient lies that close to the middle between two fp32 values
+// next to an e4m3 rounding boundary, and no 16-bit value under a scale of this rule does: all of
+// them, under every maximum of either type, were compared with the division. Otherwise
+// y * RN(1 / scale): y carries a few fp32 roundings of its own already, and 1.5 more of 2^-24 are
+// far below e4m3's half step 2^-4. Every quotient whose code is not zero has |y| >= 2^-28 (scale
+// >= 2^-17.8), so no step leaves the normal range where it counts; scales reach 7.6e35 (bf16),
+// whose reciprocal is normal. An infinite scale has no residual (it would be NaN): it keeps y * 0.
 template <bool kExact>
-__device__ __forceinline__ float divide(float y, const GroupDiv& d) {
-  float q = __fmul_rn(y, d.r);
-  if constexpr (kExact) {
-    // An infinite scale (an infinite value in the group) makes the residual NaN: keep y * 0.
-    if (d.r != 0.f) {
-      // Residual b q - y times -r: in this sign a zero keeps its own.
-      q = __fmaf_rn(__fmaf_rn(d.b, q, -y), -d.r, q);
-      q = __fmaf_rn(__fmaf_rn(d.b, q, -y), -d.r, q);
-    }
-  }
-  return q;
-}
-template <bool kExact>
-__device__ __forceinline__ uint2 codes8(const float (&y)[8], const GroupDiv& d) {
+__device__ __forceinline__ uint2 codes8(const float (&y)[8], float scale) {
+  const float r = __frcp_rn(scale);
+  const uint64_t r2 = f32x2(r, r), nr2 = f32x2(-r, -r), b2 = f32x2(scale, scale);
+  const bool correct = kExact && r != 0.f;
   uint32_t c[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    c[i] = cvt_e4m3x2(divide<kExact>(y[2 * i], d), divide<kExact>(y[2 * i + 1], d));
+  for (int i = 0; i < 4; ++i) {
+    const uint64_t v = f32x2(y[2 * i], y[2 * i + 1]);
+    uint64_t q = mul_f32x2(v, r2);
+    // Residual b q - y times -r: in this sign a zero keeps its own.
+    if (correct) q = fma_f32x2(fma_f32x2(b2, q, f32x2(-y[2 * i], -y[2 * i + 1])), nr2, q);
+    const float2 f = split_f32x2(q);
+    c[i] = cvt_e4m3x2(f.x, f.y);
+  }
   return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+}
+// One code, for rows that are not 16-byte vectors.
+template <bool kExact>
+__device__ __forceinline__ uint8_t code1(float y, float scale) {
+  const float r = __frcp_rn(scale);
+  float q = __fmul_rn(y, r);
+  if (kExact && r != 0.f) q = __fmaf_rn(__fmaf_rn(scale, q, -y), -r, q);
+  return static_cast<uint8_t>(cvt_e4m3x2(q, 0.f) & 0xFFu);
+}
+
+// Division of n < 2^31 by a divisor fixed at launch: n / d = (mulhi(n, mul) + n) >> shift
+// (T. Granlund, P. L. Montgomery, "Division by invariant integers using multiplication", 1994).
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t shift = 0;
+  while ((uint64_t(1) << shift) < d) ++shift;
+  const uint64_t mul = ((uint64_t(1) << 32) * ((uint64_t(1) << shift) - d)) / d + 1;
+  return FastDiv{d, static_cast<uint32_t>(mul), shift};
+}
+__device__ __forceinline__ uint32_t div_by(uint32_t n, const FastDiv& f) {
+  return (__umulhi(n, f.mul) + n) >> f.shift;
 }
 
 }  // namespace tfb
