@@ -5,6 +5,9 @@ arch=compute_100a,code=sm_100a``) into ``_build/`` and linked into one shared li
 CUDA runtime linked statically, so the library has no dependency beyond the driver. The C ABI
 it exports is declared in ``include/tokenforge_b200.h``.
 
+Beside it, ``lib/fp8_host.so`` is the host fast path of the FP8 operators (``csrc/host``), a
+CPython extension compiled by the host compiler against PyTorch's headers.
+
     python -m tokenforge_b200._build [--force] [--verbose]
 """
 
@@ -16,6 +19,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -23,6 +27,8 @@ ROOT = PKG.parent
 CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "lib" / "libtokenforge_b200.so"
+HOST_SRC = CSRC / "host" / "fp8_host.cpp"
+HOST_LIB = PKG / "lib" / "fp8_host.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -78,6 +84,33 @@ def _compile(src: Path, verbose: bool) -> Path:
     return obj
 
 
+def _build_host(force: bool) -> None:
+    """The CPython extension: linked against PyTorch and the kernel library next to it."""
+    if not force and not _stale(HOST_LIB, [HOST_SRC, LIB, *INCLUDE.glob("*.h")]):
+        return
+    import torch
+
+    cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: a C++ compiler is required to build tokenforge_b200")
+    pt = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = HOST_LIB.with_suffix(".so.tmp")
+    cmd = [
+        cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+        f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        f"-I{pt / 'include'}", f"-I{pt / 'include/torch/csrc/api/include'}",
+        f"-I{cuda / 'include'}", f"-I{sysconfig.get_paths()['include']}", str(HOST_SRC),
+        "-o", str(tmp), f"-L{LIB.parent}", "-ltokenforge_b200", f"-L{pt / 'lib'}",
+        "-ltorch_python", "-ltorch_cuda", "-ltorch_cpu", "-ltorch", "-lc10", "-lc10_cuda",
+        "-Wl,-rpath,$ORIGIN",
+    ]  # fmt: skip
+    proc = subprocess.run(cmd, capture_output=True, text=True)
+    if proc.returncode != 0:
+        raise RuntimeError(f"{cxx} failed on {HOST_SRC.name}:\n{proc.stderr}")
+    os.replace(tmp, HOST_LIB)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
     """Compile and link the kernel library if any source is newer than it. Returns its path."""
     BUILD.mkdir(exist_ok=True)
@@ -96,6 +129,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         if proc.returncode != 0:
             raise RuntimeError(f"link failed:\n{proc.stderr}")
         os.replace(tmp, LIB)
+    _build_host(force)
     return LIB
 
 

@@ -8,12 +8,15 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import importlib.machinery
+import importlib.util
 import threading
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtokenforge_b200.so"
+HOST_PATH = LIB_PATH.with_name("fp8_host.so")
 
 TF_OK = 0
 TF_ERR_INVALID_ARG = 1
@@ -182,6 +185,22 @@ def lib() -> ctypes.CDLL:
             fn.restype = res
             fn.argtypes = args
     return handle
+
+
+@functools.cache
+def fp8_host():  # type: ignore[no-untyped-def]
+    """The host fast path of the FP8 operators (``csrc/host/fp8_host.cpp``)."""
+    lib()  # the kernel library it is linked against, with its own message if it is missing
+    if not HOST_PATH.exists():
+        raise ImportError(
+            f"tokenforge_b200 host extension not found at {HOST_PATH}; build it with "
+            "`python -m tokenforge_b200._build`"
+        )
+    loader = importlib.machinery.ExtensionFileLoader("fp8_host", str(HOST_PATH))
+    spec = importlib.util.spec_from_file_location("fp8_host", str(HOST_PATH), loader=loader)
+    module = importlib.util.module_from_spec(spec)
+    loader.exec_module(module)
+    return module
 
 
 def status_string(status: int) -> str:

@@ -8,6 +8,10 @@ Four operators, in the order a decoder layer runs them around its attention:
 * :func:`silu_mul_fp8_quant`    SiLU-gated product of a gate_up output + e4m3 quantization,
 * :func:`e4m3_quant_groups`     the quantization alone (an attention output).
 
+Each function first offers its arguments to the host fast path (``csrc/host/fp8_host.cpp``: one
+C++ call that checks, allocates and launches); what that does not take as the plain case (strided
+or misaligned tensors, another current device, anything wrong) is handled, or refused, below.
+
 The functions here are the direct launchers; :mod:`tokenforge_b200.ops` exports them and registers
 the same names as ``torch.ops.tokenforge.*`` with fakes for tracing. Calls enqueue on the current
 CUDA stream of the inputs' device; outputs come from PyTorch's caching allocator.
@@ -22,6 +26,16 @@ import torch
 from tokenforge_b200 import _lib
 
 GROUP = 128
+
+_fast = None  # the host fast path's module, loaded by the first call
+
+
+def _load_fast():  # type: ignore[no-untyped-def]
+    global _fast
+    _fast = _lib.fp8_host()
+    return _fast
+
+
 _DTYPES = {torch.float16: _lib.TF_DTYPE_FP16, torch.bfloat16: _lib.TF_DTYPE_BF16}
 _CODES = (torch.float8_e4m3fn, torch.uint8)
 
@@ -44,10 +58,6 @@ def _same_gpu(index: int, t: torch.Tensor, name: str) -> None:
     if t.get_device() != index:
         if _gpu_index(t, name) != index:
             raise ValueError(f"{name} is on {t.device}, expected cuda:{index}")
-
-
-# The calls on few tokens take the host longer than the GPU, so the functions below look at every
-# tensor once and allocate with the cheapest calls (empty_like of a contiguous tensor, new_empty).
 
 
 def _rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
@@ -90,6 +100,9 @@ def add_rmsnorm_fp8_quant(
     ``group_size=0``. ``residual=None``: h is x itself. Between h and the codes nothing is
     rounded to 16 bits, unlike :func:`ops.rmsnorm_fp8_quant`, which rounds as the reference does.
     """
+    out = (_fast or _load_fast()).add_rmsnorm(x, residual, weight, eps, group_size)
+    if out is not None:
+        return out
     h = x.shape[-1] if x.dim() else 0
     dtype = _stream_dtype(x, "x")
     if h == 0:
@@ -136,6 +149,9 @@ def silu_mul_fp8_quant(
     """``y = silu(gate) * up`` of ``gate_up [..., 2I]`` (fp16 or bf16) in fp32, and its e4m3 codes:
     ``(q [..., I], scale [..., ceil(I / 128)] fp32)``; ``scale [..., 1]`` with ``group_size=0``.
     """
+    out = (_fast or _load_fast()).silu_mul(gate_up, group_size)
+    if out is not None:
+        return out
     dtype = _stream_dtype(gate_up, "gate_up")
     width = gate_up.shape[-1] if gate_up.dim() else 0
     if width == 0 or width % 2:
@@ -163,6 +179,9 @@ def e4m3_quant_groups(x: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """e4m3 codes of ``x [..., C]`` (fp16 or bf16) with a scale per 128 columns, exactly
     ``e4m3(x / scale)`` with the fp32 division's rounding: ``(q, scale [..., ceil(C / 128)])``.
     One scale per row: :func:`ops.e4m3_quant_rows`."""
+    out = (_fast or _load_fast()).quant_groups(x)
+    if out is not None:
+        return out
     dtype = _stream_dtype(x, "x")
     c = x.shape[-1] if x.dim() else 0
     if c == 0:
@@ -196,6 +215,9 @@ def w8a8_block_linear(
     ``[N, K]`` e4m3, w_scale fp32 ``[ceil(N / 128), ceil(K / 128)]``, bias ``[N]`` in the output
     type (fp16 or bf16). K must be a multiple of 16.
     """
+    y = (_fast or _load_fast()).block_linear(xq, x_scale, wq, w_scale, bias, out_dtype)
+    if y is not None:
+        return y
     if xq.dtype not in _CODES:
         raise TypeError(f"xq must be float8_e4m3fn (or its uint8 codes), got {xq.dtype}")
     if wq.dtype not in _CODES:
