@@ -326,7 +326,12 @@ TF_API int tf_e4m3_quant_rows(const uint16_t* y, int64_t R, int64_t C, int64_t l
  * y in fp32, never rounded to the stream's type. A NaN in a group makes its scale and all its
  * codes NaN; an infinite value makes the scale infinite, its own code NaN and the others 0.
  * Rows need not be aligned and row strides may be any number of elements >= the row; 16-byte
- * aligned rows whose stride and length are multiples of 8 elements run several times faster. */
+ * aligned rows whose stride and length are multiples of 8 elements run several times faster.
+ *
+ * These kernels are always launched as programmatic dependents of the kernel before them on the
+ * stream: their CTAs may become resident before it has finished, but they access memory only
+ * after it has. With TF_LAUNCH_PDL set, the norm's weight, and wq and w_scale at decode sizes,
+ * are read before that, under the condition stated there. */
 enum { TF_DTYPE_FP16 = 0, TF_DTYPE_BF16 = 1 };
 
 /* residual_out = dtype(x + residual);  h = residual_out in fp32;

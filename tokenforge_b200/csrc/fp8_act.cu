@@ -81,7 +81,8 @@ struct NormArgs {
   float* scale;
   int64_t T, H, ldx, ldr, ldo;
   float eps;
-  int group;  // 128, or 0 for one scale per row
+  int group;      // 128, or 0 for one scale per row
+  int w_early;    // the weight may be read before the preceding kernel has finished
 };
 
 // CTAs walk the rows (row, row + grid, ...), VPT 16-byte vectors of a row per thread, the row's sum
@@ -101,6 +102,7 @@ __global__ void __launch_bounds__(512, norm_ctas(VPT)) add_rmsnorm_row_kernel(co
   const int groups = (nvec + kGroupVecs - 1) / kGroupVecs;
   const uint4* w = reinterpret_cast<const uint4*>(a.weight);
   uint4 g[VPT], x[VPT], r[VPT];
+  if (!a.w_early) pdl_begin();
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int j = tid + nt * i;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(512, norm_ctas(VPT)) add_rmsnorm_row_kernel(co
     }
   };
   // x and the residual (and the outputs) may belong to the preceding kernel on the stream.
-  pdl_wait();
+  if (a.w_early) pdl_begin();
   if (kAhead) load(blockIdx.x);
   int phase = 0;
   for (int64_t row = blockIdx.x; row < a.T; row += gridDim.x, phase ^= 1) {
@@ -199,11 +201,11 @@ __global__ void __launch_bounds__(512) add_rmsnorm_group_kernel(const NormArgs a
   T* sr = reinterpret_cast<T*>(a.sum_out) + row * a.ldo;
   auto column = [&](int p, int j) { return (warp + nw * p) * kGroup + lane + 32 * j; };
   float g[GP][4], y[GP][4];
+  pdl_begin();
 #pragma unroll
   for (int p = 0; p < GP; ++p)
 #pragma unroll
     for (int j = 0; j < 4; ++j) g[p][j] = column(p, j) < H ? widen(w[column(p, j)]) : 0.f;
-  pdl_wait();
 #pragma unroll
   for (int p = 0; p < GP; ++p)
 #pragma unroll
@@ -270,7 +272,7 @@ __global__ void __launch_bounds__(512) add_rmsnorm_any_kernel(const NormArgs a) 
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
   const T* rr = reinterpret_cast<const T*>(a.residual) + row * a.ldr;
   T* sr = reinterpret_cast<T*>(a.sum_out) + row * a.ldo;
-  pdl_wait();
+  pdl_begin();
   float sumsq = 0.f;
   for (int64_t c = threadIdx.x; c < a.H; c += blockDim.x) {
     float f = widen(xr[c]);
@@ -373,7 +375,7 @@ __global__ void __launch_bounds__(256) quant_groups_kernel(const GroupArgs a, co
   const int groups = static_cast<int>(per_row.d) / kGroupVecs;
   const uint32_t total = static_cast<uint32_t>(a.R) * per_row.d;
   const T* x = reinterpret_cast<const T*>(a.x);
-  pdl_wait();
+  pdl_begin();
   const uint32_t base = blockIdx.x * (256 * U) + threadIdx.x;
   typename Source<T>::Raw raw[U];
 #pragma unroll
@@ -407,7 +409,7 @@ __global__ void __launch_bounds__(256) quant_groups_any_kernel(const GroupArgs a
   const uint32_t groups = per_row.d;
   const uint32_t id = blockIdx.x * 8 + (threadIdx.x >> 5);
   const int lane = threadIdx.x & 31;
-  pdl_wait();
+  pdl_begin();
   if (id >= static_cast<uint32_t>(a.R) * groups) return;
   const int64_t row = div_by(id, per_row), g = id - static_cast<uint32_t>(row) * groups;
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
@@ -434,7 +436,7 @@ template <typename T, template <typename> class Source, int VPT>
 __global__ void __launch_bounds__(1024) quant_row_kernel(const GroupArgs a) {
   __shared__ uint32_t sh_max[2][32];
   const int nvec = static_cast<int>(a.C / 8), tid = threadIdx.x, nt = blockDim.x;
-  pdl_wait();
+  pdl_begin();
   typename Source<T>::Raw raw[VPT];
   auto load = [&](int64_t row) {
     const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
@@ -466,7 +468,7 @@ __global__ void __launch_bounds__(1024) quant_row_any_kernel(const GroupArgs a) 
   __shared__ uint32_t sh_max[32];
   const int64_t row = blockIdx.x;
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ldx;
-  pdl_wait();
+  pdl_begin();
   uint32_t m = 0;
   for (int64_t c = threadIdx.x; c < a.C; c += blockDim.x)
     m = max(m, abs_bits(Source<T>::one(xr, c, a.C)));
@@ -489,7 +491,7 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, cudaStream_t stre
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
+  cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a...);
   if (e != cudaSuccess) {
     last_cuda_error() = static_cast<int>(e);
@@ -595,7 +597,8 @@ extern "C" int tf_add_rmsnorm_fp8_quant(const uint16_t* x, int64_t T, int64_t H,
     return TF_ERR_INVALID_ARG;
   if (residual && (ldr < H || ldo < H)) return TF_ERR_INVALID_ARG;
   const NormArgs a{x, residual, weight, residual_out, q, scale_out, T, H, ldx,
-                   residual ? ldr : 0, residual ? ldo : 0, eps, group_size};
+                   residual ? ldr : 0, residual ? ldo : 0, eps, group_size,
+                   (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == TF_DTYPE_FP16 ? launch_norm<__half>(a, s) : launch_norm<__nv_bfloat16>(a, s);
 }

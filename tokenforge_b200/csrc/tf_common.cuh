@@ -89,6 +89,14 @@ __device__ __forceinline__ void pdl_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;");
 }
 
+// The start of a kernel that is always launched as a programmatic dependent: its CTAs may become
+// resident while the preceding kernel's last ones run, touch nothing of its memory before they
+// have all finished, and let the next kernel on the stream do the same.
+__device__ __forceinline__ void pdl_begin() {
+  pdl_wait();
+  pdl_launch_dependents();
+}
+
 // fp32 pair -> e4m3x2, round-to-nearest-even with saturation to +-448 (NaN stays NaN).
 __device__ __forceinline__ uint16_t cvt_e4m3x2(float lo, float hi) {
   uint16_t r;

@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // The activations (and y) may belong to the preceding kernel on the stream.
-  pdl_wait();
+  pdl_begin();
 
   // This pair's tiles, and its share of K in each: with splits > 1 a cluster has one tile.
   const int kb0 = kb_begin(p, share), kb1 = kb_begin(p, share + 1);
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(Swap<kCols>::kThreads, Swap<kCols>::kCtasPerSm
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   // The activations (and y) may belong to the preceding kernel on the stream.
-  pdl_wait();
+  pdl_begin();
 
   // This CTA's tiles, and its share of K in each: with splits > 1 a cluster has one tile.
   const int share = p.splits > 1 ? static_cast<int>(cluster_cta_rank()) : 0;
@@ -906,12 +906,9 @@ cudaLaunchConfig_t tc_config(unsigned grid, int threads, int smem, int cluster, 
   attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.numAttrs = 1;
-  if (launch_flags() & TF_LAUNCH_PDL) {
-    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[1].val.programmaticStreamSerializationAllowed = 1;
-    cfg.numAttrs = 2;
-  }
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 2;
   return cfg;
 }
 

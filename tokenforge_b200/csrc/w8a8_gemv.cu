@@ -40,7 +40,8 @@ struct Stage {
 };
 
 template <typename T>
-__global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Args a, int wk) {
+__global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Args a, int wk,
+                                                                  int w_early) {
   __shared__ float part[kWarps][kTokens][kRows + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -60,6 +61,7 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Arg
   const uint4 zero = make_uint4(0, 0, 0, 0);
 
   Stage st[kStages];
+  if (!w_early) pdl_begin();
   auto load_w = [&](Stage& s, int b) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -82,8 +84,8 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Arg
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
     if (kw + s * wk < kblocks) load_w(st[s], kw + s * wk);
-  // The weights are constant; the activations may belong to the preceding kernel.
-  pdl_wait();
+  // The activations may belong to the preceding kernel.
+  if (w_early) pdl_begin();
 #pragma unroll
   for (int s = 0; s < kStages; ++s)
     if (kw + s * wk < kblocks) load_x(st[s], kw + s * wk);
@@ -119,7 +121,6 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Arg
   part[warp][2 * t][g + 8] = acc[2];
   part[warp][2 * t + 1][g + 8] = acc[3];
   __syncthreads();
-  pdl_launch_dependents();
   // Outputs of the CTA: wn tiles x 8 tokens x 16 rows.
   for (int i = threadIdx.x; i < wn * kTokens * kRows; i += 32 * kWarps) {
     const int r = i % kRows, tl = (i / kRows) % wn, m = i / (kRows * wn);
@@ -151,10 +152,12 @@ int launch_w8a8_gemv(const W8A8Args& a, cudaStream_t stream) {
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
+  cfg.numAttrs = 1;
+  const int w_early = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
   const cudaError_t e = a.dtype == TF_DTYPE_FP16
-                            ? cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__half>, a, wk)
-                            : cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__nv_bfloat16>, a, wk);
+                            ? cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__half>, a, wk, w_early)
+                            : cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__nv_bfloat16>, a, wk,
+                                                 w_early);
   if (e != cudaSuccess) {
     last_cuda_error() = static_cast<int>(e);
     return TF_ERR_CUDA;
