@@ -19,5 +19,9 @@ extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int
   if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL) return TF_ERR_TOO_LARGE;
   const W8A8Args a{xq, x_scale, wq, w_scale, bias, y, M, N, K, ldx, ld_xs, ldy, dtype};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return M <= 8 ? launch_w8a8_gemv(a, s) : launch_w8a8_tc(a, s);
+  // At most 8 tokens: the warp-MMA kernel starts soonest (3584 x 3584: 6.0 against 7.2 us), the
+  // tensor-core kernel streams more weights at once (7168 x 3584: 9.5 against 10.4 us, 37888 x
+  // 3584: 24.4 against 34.8) and splits a long K over more SMs (512 x 18944: 10.5 against 18.8).
+  const bool gemv = M <= 8 && N * K <= (int64_t(20) << 20) && K <= 8192;
+  return gemv ? launch_w8a8_gemv(a, s) : launch_w8a8_tc(a, s);
 }

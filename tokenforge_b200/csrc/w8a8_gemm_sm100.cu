@@ -19,8 +19,7 @@
 //     64 columns each, hide the latency of each other's TMEM loads.
 //   w8a8_swap_kernel, weight rows as lanes, few tokens: tile of 128 weight rows x 16, 32 or 64
 //     tokens. No tensor-core rows are wasted on missing tokens, the weight stream sets the pace,
-//     and the scale of a column (token) comes from shared memory. One warp per quadrant, two
-//     CTAs per SM.
+//     and the scale of a column (token) comes from shared memory. One warp per quadrant.
 //
 // Warps: 0 TMA producer, 1 TMEM allocation and MMA issue, 2 fetches each block's scales into a
 // small ring, 3 idle; the rest promote. Persistent CTAs (pairs) walk the tiles with the token
@@ -625,7 +624,6 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 template <int kCols>
 struct Swap {
   static constexpr int kThreads = 256;
-  static constexpr int kCtasPerSm = 2;
   static constexpr int kABytes = kLanes * kBlockK;
   static constexpr int kBBytes = kCols * kBlockK;
   static constexpr int kStageBytes = kABytes + kBBytes;
@@ -633,11 +631,14 @@ struct Swap {
   static constexpr int kTmemCols = kAccs * kCols;
   using Scales = ScaleEntry<kCols>;
   static constexpr int kTail = 1024 + kAccs * static_cast<int>(sizeof(Scales)) + 512;
-  static constexpr int kStages = (112 * 1024 - kTail) / kStageBytes;
+  // More stages than fit 160 KB were slower again (37888 x 3584, 16 tokens: 25.2 us with 160 KB,
+  // 25.6 with 112, 27.1 with 220): about 1000 128-byte TMA rows in flight an SM are enough.
+  static constexpr int kBudget = 160 * 1024;
+  static constexpr int kStages = (kBudget - kTail) / kStageBytes;
   static constexpr int kRingOff = kStages * kStageBytes;
   static constexpr int kBarOff = kRingOff + kAccs * static_cast<int>(sizeof(Scales));
   static constexpr int kSmem = 1024 + kBarOff + 512;
-  static_assert(kTmemCols >= 32 && kTmemCols * kCtasPerSm <= 512, "TMEM");
+  static_assert(kTmemCols >= 32 && kTmemCols <= 512, "TMEM");
   static_assert(kLanes * kCols * 4 <= kRingOff, "exchange buffer");
 };
 
@@ -649,7 +650,7 @@ __device__ __forceinline__ void store_token(const W8A8Args& a, int64_t m, int64_
 }
 
 template <int kCols, typename T>
-__global__ void __launch_bounds__(Swap<kCols>::kThreads, Swap<kCols>::kCtasPerSm)
+__global__ void __launch_bounds__(Swap<kCols>::kThreads, 1)
     w8a8_swap_kernel(const __grid_constant__ CUtensorMap tm_w,
                      const __grid_constant__ CUtensorMap tm_x,
                      const __grid_constant__ CUtensorMap, const TcArgs p) {
@@ -940,23 +941,34 @@ int tc_prepare(TcDevice& d, TcKernel kernel, int threads, int smem, int base) {
   return TF_OK;
 }
 
-// `base`: CTAs that share a tile and a share of K (2 for the pair kernel). Picks the K split that
-// leaves the busiest cluster the fewest blocks, an exchange counted as two blocks' time; the
-// clusters of a split launch must all be resident at once.
-int tc_launch(TcDevice& d, TcKernel kernel, int threads, int smem, int base,
-              const CUtensorMap (&maps)[3], TcArgs& p, cudaStream_t stream) {
-  const int st = tc_prepare(d, kernel, threads, smem, base);
-  if (st != TF_OK) return st;
+// Estimated time of a launch in ns, fitted to measurements of 1 to 148 blocks of K on this GPU: a
+// fixed part (launch, set-up, first bytes from HBM, output), the exchange of a split, and a time
+// per block of the busiest cluster.
+struct TcCost {
+  int fixed, exchange, block;
+};
+
+struct TcSplit {
+  int splits;
+  int64_t ns;
+};
+
+// `base`: CTAs that share a tile and a share of K (2 for the pair kernel). The K split with the
+// least estimated time; the clusters of a split launch must all be resident at once.
+TcSplit tc_split(const TcDevice& d, int base, const TcCost& c, const TcArgs& p) {
   const int64_t tiles = static_cast<int64_t>(p.tok_tiles) * p.w_tiles;
-  p.splits = 1;
-  int64_t best = cdiv(tiles, std::max(1, d.clusters[base])) * p.kb_total;
+  const int64_t waves = cdiv(tiles, std::max(1, d.clusters[base]));
+  TcSplit best{1, c.fixed + waves * p.kb_total * c.block};
   for (int s = 2; s * base <= 8 && s <= p.kb_total && tiles <= d.clusters[s * base]; ++s) {
-    const int64_t cost = cdiv(p.kb_total, s) + 2;
-    if (cost < best) {
-      best = cost;
-      p.splits = s;
-    }
+    const int64_t ns = c.fixed + c.exchange + cdiv(p.kb_total, s) * c.block;
+    if (ns < best.ns) best = TcSplit{s, ns};
   }
+  return best;
+}
+
+int tc_launch(const TcDevice& d, TcKernel kernel, int threads, int smem, int base,
+              const CUtensorMap (&maps)[3], const TcArgs& p, cudaStream_t stream) {
+  const int64_t tiles = static_cast<int64_t>(p.tok_tiles) * p.w_tiles;
   const int64_t clusters = p.splits > 1 ? tiles : std::min<int64_t>(tiles, d.clusters[base]);
   cudaLaunchAttribute attr[2];
   const cudaLaunchConfig_t cfg =
@@ -1003,51 +1015,99 @@ bool tile_counts(const W8A8Args& a, int tokens, int rows, TcArgs* p) {
   return tt * wt < 0x7fffffffLL;
 }
 
+// A kernel form: its tile counts and K split for these operands on this device, and its launch.
 template <typename T>
-int launch_pair(const W8A8Args& a, cudaStream_t stream) {
-  static TcDevice devices[kMaxDevices];
-  int dev = 0;
-  const int st = current_device(&dev);
-  if (st != TF_OK) return st;
+struct PairForm {
+  static constexpr TcCost kCost{6700, 4500, 420};
+  TcDevice* device;
   TcArgs p;
-  if (!tile_counts(a, Pair::kTokens, Pair::kCols, &p)) return TF_ERR_TOO_LARGE;
-  CUtensorMap maps[3];
-  if (!make_map(&maps[0], a.xq, a.K, a.M, a.ldx, kLanes) ||
-      !make_map(&maps[1], a.wq, a.K, a.N, a.K, Pair::kCols / 2))
-    return TF_ERR_ALIGNMENT;
-  // The output goes through TMA where its rows allow it, else by plain stores.
-  p.tma_out = aligned16(a.y) && a.ldy % 8 == 0;
-  maps[2] = maps[0];
-  if (p.tma_out && !make_out_map(&maps[2], a, 32, Pair::kOutCols)) return TF_ERR_ALIGNMENT;
-  return tc_launch(devices[dev], w8a8_pair_kernel<T>, Pair::kThreads, Pair::kSmem, 2, maps, p,
-                   stream);
-}
+  int64_t ns;
+
+  int plan(const W8A8Args& a, int dev) {
+    static TcDevice devices[kMaxDevices];
+    device = &devices[dev];
+    const int st = tc_prepare(*device, w8a8_pair_kernel<T>, Pair::kThreads, Pair::kSmem, 2);
+    if (st != TF_OK) return st;
+    if (!tile_counts(a, Pair::kTokens, Pair::kCols, &p)) return TF_ERR_TOO_LARGE;
+    const TcSplit s = tc_split(*device, 2, kCost, p);
+    p.splits = s.splits;
+    ns = s.ns;
+    return TF_OK;
+  }
+  int launch(const W8A8Args& a, cudaStream_t stream) {
+    CUtensorMap maps[3];
+    if (!make_map(&maps[0], a.xq, a.K, a.M, a.ldx, kLanes) ||
+        !make_map(&maps[1], a.wq, a.K, a.N, a.K, Pair::kCols / 2))
+      return TF_ERR_ALIGNMENT;
+    // The output goes through TMA where its rows allow it, else by plain stores.
+    p.tma_out = aligned16(a.y) && a.ldy % 8 == 0;
+    maps[2] = maps[0];
+    if (p.tma_out && !make_out_map(&maps[2], a, 32, Pair::kOutCols)) return TF_ERR_ALIGNMENT;
+    return tc_launch(*device, w8a8_pair_kernel<T>, Pair::kThreads, Pair::kSmem, 2, maps, p,
+                     stream);
+  }
+};
 
 template <int kCols, typename T>
-int launch_swap(const W8A8Args& a, cudaStream_t stream) {
-  using C = Swap<kCols>;
-  static TcDevice devices[kMaxDevices];
-  int dev = 0;
-  const int st = current_device(&dev);
-  if (st != TF_OK) return st;
+struct SwapForm {
+  static constexpr TcCost kCost{4500, 2000, kCols == 64 ? 380 : 300};
+  TcDevice* device;
   TcArgs p;
-  if (!tile_counts(a, kCols, kLanes, &p)) return TF_ERR_TOO_LARGE;
-  CUtensorMap maps[3];
-  if (!make_map(&maps[0], a.wq, a.K, a.N, a.K, kLanes) ||
-      !make_map(&maps[1], a.xq, a.K, a.M, a.ldx, kCols))
-    return TF_ERR_ALIGNMENT;
-  maps[2] = maps[0];  // unused: an output row's 32 neighbours are one plain store
-  p.tma_out = 0;
-  return tc_launch(devices[dev], w8a8_swap_kernel<kCols, T>, C::kThreads, C::kSmem, 1, maps, p,
-                   stream);
+  int64_t ns;
+
+  int plan(const W8A8Args& a, int dev) {
+    using C = Swap<kCols>;
+    static TcDevice devices[kMaxDevices];
+    device = &devices[dev];
+    const int st = tc_prepare(*device, w8a8_swap_kernel<kCols, T>, C::kThreads, C::kSmem, 1);
+    if (st != TF_OK) return st;
+    if (!tile_counts(a, kCols, kLanes, &p)) return TF_ERR_TOO_LARGE;
+    const TcSplit s = tc_split(*device, 1, kCost, p);
+    p.splits = s.splits;
+    ns = s.ns;
+    return TF_OK;
+  }
+  int launch(const W8A8Args& a, cudaStream_t stream) {
+    using C = Swap<kCols>;
+    CUtensorMap maps[3];
+    if (!make_map(&maps[0], a.wq, a.K, a.N, a.K, kLanes) ||
+        !make_map(&maps[1], a.xq, a.K, a.M, a.ldx, kCols))
+      return TF_ERR_ALIGNMENT;
+    maps[2] = maps[0];  // unused: an output row's 32 neighbours are one plain store
+    p.tma_out = 0;
+    return tc_launch(*device, w8a8_swap_kernel<kCols, T>, C::kThreads, C::kSmem, 1, maps, p,
+                     stream);
+  }
+};
+
+template <typename Form>
+int run_form(const W8A8Args& a, int dev, cudaStream_t stream) {
+  Form f;
+  const int st = f.plan(a, dev);
+  return st == TF_OK ? f.launch(a, stream) : st;
 }
 
+// Up to 64 tokens: one token tile with weight rows as lanes. Above, up to 512: whichever of the
+// two forms is estimated faster; 64-token tiles fill more SMs and start sooner, pairs read the
+// weights once (128 tokens: 3584 x 3584 11.9 against 13.2 us, 37888 x 3584 52 against 36).
 template <typename T>
 int launch_tc(const W8A8Args& a, cudaStream_t stream) {
-  if (a.M <= 16) return launch_swap<16, T>(a, stream);
-  if (a.M <= 32) return launch_swap<32, T>(a, stream);
-  if (a.M <= 64) return launch_swap<64, T>(a, stream);
-  return launch_pair<T>(a, stream);
+  int dev = 0;
+  int st = current_device(&dev);
+  if (st != TF_OK) return st;
+  if (a.M <= 16) return run_form<SwapForm<16, T>>(a, dev, stream);
+  if (a.M <= 32) return run_form<SwapForm<32, T>>(a, dev, stream);
+  if (a.M <= 64) return run_form<SwapForm<64, T>>(a, dev, stream);
+  PairForm<T> pair;
+  st = pair.plan(a, dev);
+  if (st != TF_OK) return st;
+  if (a.M <= 512) {
+    SwapForm<64, T> swap;
+    st = swap.plan(a, dev);
+    if (st != TF_OK) return st;
+    if (swap.ns < pair.ns) return swap.launch(a, stream);
+  }
+  return pair.launch(a, stream);
 }
 
 }  // namespace
