@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(512, norm_ctas(VPT)) add_rmsnorm_row_kernel(co
 #pragma unroll
   for (int i = 0; i < VPT; ++i) {
     const int j = tid + nt * i;
-    g[i] = j < nvec ? __ldg(w + j) : make_uint4(0, 0, 0, 0);
+    g[i] = j < nvec ? w[j] : make_uint4(0, 0, 0, 0);
   }
   auto load = [&](int64_t row) {
     const uint4* xr = reinterpret_cast<const uint4*>(a.x + row * a.ldx);
@@ -324,7 +324,7 @@ struct SiluSource {
     uint4 g, u;
   };
   static __device__ __forceinline__ Raw load(const T* row, int64_t j, int64_t C) {
-    return Raw{ldg_stream_v4(row + 8 * j), ldg_stream_v4(row + C + 8 * j)};
+    return Raw{ld_stream_v4(row + 8 * j), ld_stream_v4(row + C + 8 * j)};
   }
   // y, and the bits of its largest magnitude.
   static __device__ __forceinline__ uint32_t value(const Raw& r, float (&y)[8]) {
@@ -346,7 +346,7 @@ struct CopySource {
     uint4 x;
   };
   static __device__ __forceinline__ Raw load(const T* row, int64_t j, int64_t) {
-    return Raw{ldg_stream_v4(row + 8 * j)};
+    return Raw{ld_stream_v4(row + 8 * j)};
   }
   // The maximum of the 16-bit patterns, two at a time: the same order as the widened values'.
   static __device__ __forceinline__ uint32_t value(const Raw& r, float (&y)[8]) {

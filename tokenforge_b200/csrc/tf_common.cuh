@@ -68,6 +68,16 @@ __device__ __forceinline__ uint4 ldg_stream_v4(const void* p) {
   return r;
 }
 
+// The same, coherent: for data that an overlapping kernel (programmatic launch) may have written.
+__device__ __forceinline__ uint4 ld_stream_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+               : "l"(p)
+               : "memory");
+  return r;
+}
+
 __device__ __forceinline__ uint4 ldg_v4(const void* p) {
   return __ldg(reinterpret_cast<const uint4*>(p));
 }

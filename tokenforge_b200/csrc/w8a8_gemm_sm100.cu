@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             if (4 * g + j < kb0 || 4 * g + j >= kb1) continue;
-            const float w = __ldg(sw + 4 * g + j);
+            const float w = sw[4 * g + j];
             if (!mbar_wait(&acc_full[it & 1u], ((it >> 1) & 1u) ^ 1u, kErrScale)) {
               ok = false;
               break;
@@ -755,7 +755,7 @@ __global__ void __launch_bounds__(Swap<kCols>::kThreads, 1)
         for (int j = 0; j < 4; ++j) {
           if (4 * g + j < kb0 || 4 * g + j >= kb1) continue;
           const uint32_t r = it % R;
-          const float w = __ldg(sw + 4 * g + j);
+          const float w = sw[4 * g + j];
           if (!mbar_wait(&acc_empty[r], ((it / R) & 1u) ^ 1u, kErrScale)) {
             ok = false;
             break;

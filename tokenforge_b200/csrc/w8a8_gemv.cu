@@ -67,10 +67,10 @@ __global__ void __launch_bounds__(32 * kWarps, 2) w8a8_gemv_kernel(const W8A8Arg
     for (int h = 0; h < 2; ++h) {
       const int64_t k = static_cast<int64_t>(b) * 128 + 64 * h;
       const bool ok = k + 16 * t < a.K;
-      s.w[0][h] = ok ? ldg_stream_v4(wr0 + k) : zero;
-      s.w[1][h] = ok ? ldg_stream_v4(wr1 + k) : zero;
+      s.w[0][h] = ok ? ld_stream_v4(wr0 + k) : zero;
+      s.w[1][h] = ok ? ld_stream_v4(wr1 + k) : zero;
     }
-    s.sw = __ldg(swr + b);
+    s.sw = swr[b];
   };
   auto load_x = [&](Stage& s, int b) {
 #pragma unroll
