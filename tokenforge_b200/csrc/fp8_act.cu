@@ -50,10 +50,10 @@ __device__ __forceinline__ float block_sum_f(float v, float* sh) {
 }
 
 __device__ __forceinline__ uint32_t max_bits8(const float (&y)[8]) {
-  uint32_t m = 0;
+  float m = fabsf(y[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(y[i]));
-  return m;
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(y[i]));
+  return abs_bits(m);
 }
 
 __device__ __forceinline__ float rstd_f(float sumsq, int64_t H, float eps) {
@@ -63,11 +63,16 @@ __device__ __forceinline__ float rstd_f(float sumsq, int64_t H, float eps) {
 // y = h * rstd * weight of one vector.
 template <typename T>
 __device__ __forceinline__ void norm8(const uint4& h, const uint4& w, float rstd, float (&y)[8]) {
-  float gw[8];
-  widen8<T>(h, y);
-  widen8<T>(w, gw);
+  const uint32_t* hp = reinterpret_cast<const uint32_t*>(&h);
+  const uint32_t* wp = reinterpret_cast<const uint32_t*>(&w);
+  const uint64_t r2 = f32x2(rstd, rstd);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) y[e] = y[e] * rstd * gw[e];
+  for (int e = 0; e < 4; ++e) {
+    const float2 a = widen2(hp[e], T()), b = widen2(wp[e], T());
+    const float2 f = split_f32x2(mul_f32x2(mul_f32x2(f32x2(a.x, a.y), r2), f32x2(b.x, b.y)));
+    y[2 * e] = f.x;
+    y[2 * e + 1] = f.y;
+  }
 }
 
 // ------------------------------------------------------------------ residual + RMSNorm + FP8
@@ -317,8 +322,8 @@ template <typename T>
 struct SiluSource {
   static constexpr bool kExact = false;
   static __device__ __forceinline__ float one(const T* row, int64_t c, int64_t C) {
-    const float g = widen(row[c]);
-    return __fdividef(g, 1.0f + __expf(-g)) * widen(row[C + c]);
+    const float g = widen(row[c]), u = widen(row[C + c]);
+    return split_f32x2(silu_mul2(make_float2(g, g), make_float2(u, u))).x;
   }
   struct Raw {
     uint4 g, u;
@@ -328,11 +333,14 @@ struct SiluSource {
   }
   // y, and the bits of its largest magnitude.
   static __device__ __forceinline__ uint32_t value(const Raw& r, float (&y)[8]) {
-    float g[8], u[8];
-    widen8<T>(r.g, g);
-    widen8<T>(r.u, u);
+    const uint32_t* g = reinterpret_cast<const uint32_t*>(&r.g);
+    const uint32_t* u = reinterpret_cast<const uint32_t*>(&r.u);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) y[e] = __fdividef(g[e], 1.0f + __expf(-g[e])) * u[e];
+    for (int e = 0; e < 4; ++e) {
+      const float2 f = split_f32x2(silu_mul2(widen2(g[e], T()), widen2(u[e], T())));
+      y[2 * e] = f.x;
+      y[2 * e + 1] = f.y;
+    }
     return max_bits8(y);
   }
 };

@@ -45,6 +45,11 @@ __device__ __forceinline__ void widen8(const uint4& v, float (&f)[8]) {
 // |y| maxima are taken on the bit patterns of |y| as unsigned integers. For finite values that
 // is the order of the values; Inf is above them and NaN above Inf, so a NaN in a group becomes
 // its maximum, its scale and (below) every code of it, as in the elementary operations.
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 __device__ __forceinline__ uint32_t abs_bits(float f) { return __float_as_uint(f) & 0x7FFFFFFFu; }
 
 // scale = max(amax / 448, 1 / (448 * 512)) with the IEEE quotient: q0 = amax * RN(1 / 448) is
@@ -57,6 +62,20 @@ __device__ __forceinline__ float scale_of_bits(uint32_t amax_bits) {
   float s = __fmul_rn(a, kInv);
   if (amax_bits < 0x7F800000u) s = __fmaf_rn(__fmaf_rn(-s, kFp8Max, a), kInv, s);
   return s < kMinScale ? kMinScale : s;
+}
+
+// y = g / (1 + exp(-g)) * u for a pair, exp(-g) = 2^(-g log2 e). The approximate exponential and
+// reciprocal are within a few units of 2^-23 each (and the rounding of -g log2 e adds |g| of
+// them, where y is small by e^-|g|). For g < -87 the quotient is 0, below 1e-36 of |u|.
+__device__ __forceinline__ uint64_t silu_mul2(float2 g, float2 u) {
+  const uint64_t x = mul_f32x2(f32x2(g.x, g.y), f32x2(-1.44269504f, -1.44269504f));
+  const float2 t = split_f32x2(x);
+  float e0, e1, r0, r1;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(t.y));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r0) : "f"(1.0f + e0));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r1) : "f"(1.0f + e1));
+  return mul_f32x2(mul_f32x2(f32x2(g.x, g.y), f32x2(r0, r1)), f32x2(u.x, u.y));
 }
 
 // Maximum over the 16 lanes of a half warp that hold one 128-column group (8 columns a lane).
