@@ -148,6 +148,14 @@ struct ScaleEntry {
   float sw[4];
 };
 
+// Where a split tile's partial sums lie in shared memory: 16-byte vector c (columns 4c .. 4c + 3)
+// of lane `row`, the lanes of one vector next to each other, so that a warp reads 512 contiguous
+// bytes of a peer (rows of a whole tile, a warp's vectors 1 KB apart, made an exchange three
+// times slower).
+__device__ __forceinline__ uint32_t part_at(int row, int c) {
+  return static_cast<uint32_t>((c * kLanes + row) * 16);
+}
+
 // The scale warp's view of one tile: lane l fetches tokens l, l + 32, ... of `kTokens`, four K
 // blocks at a time (one 16-byte load a token where rows allow it) and
 // one such group ahead of its use: fetched block by block, every eighth one (a new 32-byte
@@ -577,16 +585,15 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
   __syncwarp();
 
   if (p.splits > 1) {
-    // Partial tiles as [column][lane] in the (drained) stages. Units of 32 columns are dealt to
-    // the shares, and a share's to its two warps of a quadrant, which sum them over the shares in
-    // an order of the unit's own (its owner's share first, so that the CTAs do not all read the
-    // same one at a time).
-    float* part = reinterpret_cast<float*>(smem);
+    // Partial tiles in the (drained) stages. Units of 32 columns are dealt to the shares, and a
+    // share's to its two warps of a quadrant, which sum them over the shares in an order of the
+    // unit's own (its owner's share first, so that the CTAs do not all read the same one at a
+    // time).
 #pragma unroll
-    for (int i = 0; i < N2; ++i) {
-      const float2 v = split_f32x2(acc[i]);
-      part[(c0 + 2 * i) * kLanes + row] = v.x;
-      part[(c0 + 2 * i + 1) * kLanes + row] = v.y;
+    for (int i = 0; i < N2 / 2; ++i) {
+      const float2 f = split_f32x2(acc[2 * i]), g = split_f32x2(acc[2 * i + 1]);
+      *reinterpret_cast<float4*>(smem + part_at(row, c0 / 4 + i)) =
+          make_float4(f.x, f.y, g.x, g.y);
     }
     __syncwarp();
     cluster_barrier();
@@ -594,15 +601,20 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
       float v[32];
 #pragma unroll
       for (int e = 0; e < 32; ++e) v[e] = 0.f;
-#pragma unroll 1
+#pragma unroll 2
       for (int k = 0; k < p.splits; ++k) {
         const int from = share + k < p.splits ? share + k : share + k - p.splits;
-        const uint32_t at = map_to_rank(smem_u32(part + 32 * unit * kLanes + row), 2 * from + side);
-        float w[32];
+        const uint32_t at = map_to_rank(smem_u32(smem), 2 * from + side);
+        float4 w[8];
 #pragma unroll
-        for (int e = 0; e < 32; ++e) w[e] = ld_cluster(at + 4 * e * kLanes);
+        for (int e = 0; e < 8; ++e) w[e] = ld_cluster_v4(at + part_at(row, 8 * unit + e));
 #pragma unroll
-        for (int e = 0; e < 32; ++e) v[e] += w[e];
+        for (int e = 0; e < 8; ++e) {
+          v[4 * e] += w[e].x;
+          v[4 * e + 1] += w[e].y;
+          v[4 * e + 2] += w[e].z;
+          v[4 * e + 3] += w[e].w;
+        }
       }
       if (p.a.bias != nullptr) {
         const float mine = bias_of<T>(p.a, n0 + 32 * unit + lane);
@@ -824,15 +836,14 @@ __global__ void __launch_bounds__(Swap<kCols>::kThreads, 1)
   }
 
   if (p.splits > 1) {
-    // Partial tiles as [column][lane] in the (drained) stages; column chunks of 8 are summed by
-    // share chunk mod splits, over the shares in order.
-    float* part = reinterpret_cast<float*>(smem);
+    // Partial tiles in the (drained) stages; column chunks of 8 are summed by share chunk mod
+    // splits, over the shares in order.
     if (warp >= 4) {
 #pragma unroll
-      for (int i = 0; i < N2; ++i) {
-        const float2 v = split_f32x2(acc[i]);
-        part[2 * i * kLanes + row] = v.x;
-        part[(2 * i + 1) * kLanes + row] = v.y;
+      for (int i = 0; i < N2 / 2; ++i) {
+        const float2 f = split_f32x2(acc[2 * i]), g = split_f32x2(acc[2 * i + 1]);
+        *reinterpret_cast<float4*>(smem + part_at(row, i)) =
+            make_float4(f.x, f.y, g.x, g.y);
       }
     }
     __syncwarp();
@@ -840,10 +851,17 @@ __global__ void __launch_bounds__(Swap<kCols>::kThreads, 1)
     if (warp >= 4) {
       for (int c = share; c < kCols / 8; c += p.splits) {
         float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
         for (int k = 0; k < p.splits; ++k) {
-          const uint32_t at = map_to_rank(smem_u32(part + 8 * c * kLanes + row), k);
+          const uint32_t at = map_to_rank(smem_u32(smem), k);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += ld_cluster(at + 4 * e * kLanes);
+          for (int e = 0; e < 2; ++e) {
+            const float4 w = ld_cluster_v4(at + part_at(row, 2 * c + e));
+            v[4 * e] += w.x;
+            v[4 * e + 1] += w.y;
+            v[4 * e + 2] += w.z;
+            v[4 * e + 3] += w.w;
+          }
         }
         if (n < p.a.N) {
 #pragma unroll
@@ -1018,7 +1036,7 @@ bool tile_counts(const W8A8Args& a, int tokens, int rows, TcArgs* p) {
 // A kernel form: its tile counts and K split for these operands on this device, and its launch.
 template <typename T>
 struct PairForm {
-  static constexpr TcCost kCost{6700, 4500, 420};
+  static constexpr TcCost kCost{5400, 4600, 420};
   TcDevice* device;
   TcArgs p;
   int64_t ns;
