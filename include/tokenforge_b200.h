@@ -358,7 +358,7 @@ TF_API int tf_e4m3_quant_groups(const uint16_t* x, int64_t R, int64_t C, int64_t
  * xq [M, K] row stride ldx bytes; x_scale [M, ceil(K / 128)] row stride ld_xs floats;
  * wq [N, K] contiguous; w_scale [ceil(N / 128), ceil(K / 128)] contiguous; bias dtype [N] or
  * NULL; y dtype [M, N] row stride ldy. K and ldx must be multiples of 16, xq and wq 16-byte
- * aligned; any M >= 0 and N >= 1. No workspace; results do not depend on timing: the same call
+ * aligned; any M >= 0 and N >= 1, each size at most 2^30. No workspace; results do not depend on timing: the same call
  * gives the same bits. */
 TF_API int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
                                 const float* x_scale, int64_t ld_xs, const uint8_t* wq,

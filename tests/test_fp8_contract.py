@@ -177,6 +177,8 @@ def _abi_linear(m=1, k=128, ldx=128, ldxs=1, n=128, dtype=0, ldy=128, xq=16, wq=
         ({"wq": 24}, _lib.TF_ERR_ALIGNMENT),
         ({"ldx": 136}, _lib.TF_ERR_ALIGNMENT),
         ({"m": 0}, _lib.TF_OK),
+        ({"m": (1 << 30) + 1}, _lib.TF_ERR_TOO_LARGE),
+        ({"n": (1 << 30) + 1, "ldy": (1 << 30) + 1}, _lib.TF_ERR_TOO_LARGE),
     ],
 )
 def test_abi_linear_status(change, status) -> None:  # type: ignore[no-untyped-def]

@@ -502,3 +502,61 @@ def test_e4m3_per_row_codes_feed_the_w4a16_linear(device: torch.device) -> None:
     y64, mag = a @ deq.t(), a.abs() @ deq.abs().t()
     tol = 2.0**-11 * y64.abs() + 700 * 2.0**-23 * mag + 2.0**-25
     assert bool(((y.double() - y64).abs() <= tol).all())
+
+
+def test_host_threads_on_streams_of_their_own(device: torch.device) -> None:
+    """Four host threads, a stream each, through every kernel form at once."""
+    import threading
+
+    p = pack_w8a8_block(torch.randn((1000, 528), generator=_gen(9), device=device))
+    xs = [_stream(m, 528, torch.bfloat16, m, device) for m in (1, 20, 40, 300)]
+
+    def chain(x):  # type: ignore[no-untyped-def]
+        q, s = ops.e4m3_quant_groups(x)
+        return ops.w8a8_block_linear(q, s, p.wq, p.w_scale, None, torch.bfloat16)
+
+    want = [chain(x) for x in xs]
+    torch.cuda.synchronize()
+    same = []
+
+    def work() -> None:
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(20):
+                got = [chain(x) for x in xs]
+            stream.synchronize()
+            same.append(all(torch.equal(a, b) for a, b in zip(got, want)))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True] * 4
+    assert _lib.device_error() == 0
+
+
+def test_plain_and_careful_host_paths_agree(device: torch.device) -> None:
+    """One-dimensional inputs, a Parameter as weight, an integer eps, a tensor subclass and a
+    misaligned view give what the packed tensors give, whichever host path takes them."""
+    class Sub(torch.Tensor):
+        pass
+
+    x = _stream(3, 640, torch.float16, 30, device)
+    w = torch.nn.Parameter(torch.ones(640, dtype=torch.float16, device=device))
+    q, s, h = ops.add_rmsnorm_fp8_quant(x, x, w, 1.0)
+    q1, s1, h1 = ops.add_rmsnorm_fp8_quant(x, x, w, 1)
+    assert torch.equal(q.view(torch.uint8), q1.view(torch.uint8)) and torch.equal(s, s1)
+    q1, s1, h1 = ops.add_rmsnorm_fp8_quant(x[1], x[1], w, 1.0)
+    assert q1.shape == (640,) and s1.shape == (5,) and torch.equal(h1, h[1])
+    assert torch.equal(q1.view(torch.uint8), q[1].view(torch.uint8)) and torch.equal(s1, s[1])
+    q2, s2 = ops.e4m3_quant_groups(x.as_subclass(Sub))
+    q3, s3 = ops.e4m3_quant_groups(x)
+    assert torch.equal(q2.view(torch.uint8), q3.view(torch.uint8)) and torch.equal(s2, s3)
+    p = pack_w8a8_block(torch.randn((200, 640), generator=_gen(31), device=device))
+    y = ops.w8a8_block_linear(q, s, p.wq, p.w_scale)
+    assert torch.equal(ops.w8a8_block_linear(q[2], s[2], p.wq, p.w_scale), y[2])
+    buf = torch.zeros(3 * 640 + 4, dtype=torch.uint8, device=device)
+    off = buf[4:].view(3, 640)
+    off.copy_(q.view(torch.uint8))
+    assert torch.equal(ops.w8a8_block_linear(off, s, p.wq, p.w_scale), y)

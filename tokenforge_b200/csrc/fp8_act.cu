@@ -577,7 +577,7 @@ int launch_rows(const GroupArgs& a, cudaStream_t stream) {
   const int64_t nvec = a.C / 8;
   if (!vec_rows(a) || nvec > 4096)
     return launch(quant_row_any_kernel<T, Source>, a.R, 1024, stream, a);
-  const int vpt = nvec <= 1024 ? 1 : nvec <= 2048 ? 2 : nvec <= 3072 ? 3 : 4;
+  const int vpt = static_cast<int>(cdiv(nvec, 1024));
   const int threads = static_cast<int>(cdiv(cdiv(nvec, vpt), 32) * 32);
   const int64_t grid = std::min<int64_t>(a.R, 148 * (1024 / threads));
   switch (vpt) {

@@ -16,7 +16,9 @@ extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int
   if (!xq || !x_scale || !wq || !w_scale || !y || ldx < K || ld_xs < cdiv(K, 128) || ldy < N)
     return TF_ERR_INVALID_ARG;
   if (!aligned16(xq) || !aligned16(wq) || ldx % 16 != 0) return TF_ERR_ALIGNMENT;
-  if (M > 0x7fffffffLL || N > 0x7fffffffLL || K > 0x7fffffffLL) return TF_ERR_TOO_LARGE;
+  // Tile coordinates are 32-bit numbers.
+  constexpr int64_t kMost = int64_t(1) << 30;
+  if (M > kMost || N > kMost || K > kMost) return TF_ERR_TOO_LARGE;
   const W8A8Args a{xq, x_scale, wq, w_scale, bias, y, M, N, K, ldx, ld_xs, ldy, dtype};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   // At most 8 tokens: the warp-MMA kernel starts soonest (3584 x 3584: 6.0 against 7.2 us), the
