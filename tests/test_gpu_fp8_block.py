@@ -81,6 +81,11 @@ LINEAR = [
     (64, 3584, 18944), (65, 257, 400), (100, 3584, 3584), (128, 128, 128), (129, 385, 1168),
     (200, 4608, 3584), (256, 3584, 2368), (257, 1025, 272), (500, 100, 16), (1000, 1000, 1040),
     (1024, 3584, 3584), (1300, 2368, 3584), (2049, 513, 528),
+    # Ragged sizes that are too large for the warp-MMA kernel: each tensor-core form, one and
+    # several token tiles, K split and not.
+    (5, 1003, 9232), (12, 5003, 2064), (16, 129, 16400), (17, 3601, 2576), (32, 20011, 144),
+    (48, 2005, 4112), (64, 40001, 272), (70, 1999, 2064), (127, 3000, 1040), (130, 9001, 528),
+    (333, 4613, 2960), (400, 515, 8208), (700, 2051, 1040), (1030, 777, 4112), (3000, 2050, 272),
 ]
 
 
@@ -95,11 +100,11 @@ def test_linear(m: int, n: int, k: int, dtype: torch.dtype, device: torch.device
     assert torch.equal(y, ops.w8a8_block_linear(*args, dtype)), "a second call differs"
 
 
+@pytest.mark.parametrize("n, k", [(264, 416), (2056, 2576)])
 @pytest.mark.parametrize("m", [1, 4, 40, 300])
-def test_linear_layouts(m: int, device: torch.device) -> None:
+def test_linear_layouts(m: int, n: int, k: int, device: torch.device) -> None:
     """Leading dimensions, rows and scales cut out of wider tensors, misaligned and uint8 codes,
     a bias with a stride, an x expanded over its rows."""
-    n, k = 264, 416
     xq, xs, wq, ws, b = _linear_inputs(m, n, k, torch.float16, True, device)
     y = ops.w8a8_block_linear(xq, xs, wq, ws, b)
     same = [
@@ -124,10 +129,12 @@ def test_linear_layouts(m: int, device: torch.device) -> None:
         ops.w8a8_block_linear(xq, xs, buf, ws, b)
 
 
+@pytest.mark.parametrize("n, k, ldy", [(200, 272, 216), (200, 272, 213), (2050, 2576, 2056),
+                                       (2050, 2576, 2061), (1999, 4112, 2000)])
 @pytest.mark.parametrize("m", [1, 8, 24, 64, 130, 300])
-def test_linear_writes_its_rows_only(m: int, device: torch.device) -> None:
+def test_linear_writes_its_rows_only(m: int, n: int, k: int, ldy: int,
+                                     device: torch.device) -> None:
     """C ABI with an output wider than N and rows behind the last token."""
-    n, k, ldy = 200, 272, 216
     xq, xs, wq, ws, _ = _linear_inputs(m, n, k, torch.float16, False, device)
     y = torch.full((m + 4, ldy), 7.0, dtype=torch.float16, device=device)
     lib = _lib.lib()
@@ -139,11 +146,11 @@ def test_linear_writes_its_rows_only(m: int, device: torch.device) -> None:
     assert bool((y[m:] == 7).all()) and bool((y[:, n:] == 7).all())
 
 
+@pytest.mark.parametrize("n, k", [(256, 384), (2048, 2560)])
 @pytest.mark.parametrize("m", [1, 8, 48, 200])
-def test_linear_special_values(m: int, device: torch.device) -> None:
+def test_linear_special_values(m: int, n: int, k: int, device: torch.device) -> None:
     """A NaN code or scale reaches its own row (or column) alone; a zero scale and zero codes
     give 0; an overflowing sum gives the output type's infinity."""
-    n, k = 256, 384
     xq, xs, wq, ws, _ = _linear_inputs(m, n, k, torch.float16, False, device)
     xq = xq.clone().view(torch.uint8)
     xq[m // 2, 130] = 0x7F

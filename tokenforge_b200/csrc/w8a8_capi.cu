@@ -21,9 +21,14 @@ extern "C" int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int
   if (M > kMost || N > kMost || K > kMost) return TF_ERR_TOO_LARGE;
   const W8A8Args a{xq, x_scale, wq, w_scale, bias, y, M, N, K, ldx, ld_xs, ldy, dtype};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  // At most 8 tokens: the warp-MMA kernel starts soonest (3584 x 3584: 6.0 against 7.2 us), the
-  // tensor-core kernel streams more weights at once (7168 x 3584: 9.5 against 10.4 us, 37888 x
-  // 3584: 24.4 against 34.8) and splits a long K over more SMs (512 x 18944: 10.5 against 18.8).
-  const bool gemv = M <= 8 && N * K <= (int64_t(20) << 20) && K <= 8192;
+  // The warp-MMA kernel starts soonest and needs no tensor maps; the tensor-core kernels stream
+  // more weights at once, read them once for more tokens and split a long K over more SMs. Up to
+  // 8 tokens it takes weights of 20 MB (3584 x 3584: 6.0 against 7.2 us; 7168 x 3584: 10.4 against
+  // 9.5; 512 x 18944: 18.8 against 10.5). More tokens read the weights again, 8 at a time, from
+  // L2: up to 10 MB of such reads (64 x 1000 x 1008: 4.7 against 5.8 us, 16 x 2048 x 2048: 4.0
+  // against 6.0, 16 x 3584 x 3584: 10.0 against 7.4).
+  const int64_t passes = cdiv(M, 8);
+  const bool gemv = K <= 8192 && M <= 2048 &&
+                    passes * N * K <= (int64_t(passes == 1 ? 20 : 10) << 20);
   return gemv ? launch_w8a8_gemv(a, s) : launch_w8a8_tc(a, s);
 }
