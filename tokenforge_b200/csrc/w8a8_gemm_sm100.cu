@@ -10,24 +10,29 @@
 // lets the tensor core fill the next block while one is promoted.
 //
 // Two kernels, by which operand gives the accumulator's 128 lanes:
-//   w8a8_pair_kernel, tokens as lanes, M > 64: a CTA pair (two SMs, cta_group::2 MMAs) computes
-//     256 tokens x 256 weight rows, each CTA holding 128 tokens' sums and half of the weight rows
-//     in shared memory, so a block costs an SM 32 KB of L2 traffic instead of the 48 KB of a
-//     single CTA's 128 x 256 tile (measured: that form stopped at 2180 TFLOP/s even without
-//     promotion). A lane is a token, so a block's scale is one number per thread and 64
-//     columns, and promotion costs one packed FMA per two values. Four warps per TMEM quadrant,
-//     64 columns each, hide the latency of each other's TMEM loads.
+//   w8a8_pair_kernel, tokens as lanes, many tokens: a CTA pair (two SMs, cta_group::2 MMAs)
+//     computes 256 tokens x 256 weight rows, each CTA holding 128 tokens' sums and half of the
+//     weight rows in shared memory, so a block costs an SM 32 KB of L2 traffic instead of the 48 KB
+//     of a single CTA's 128 x 256 tile (which stopped at 2180 TFLOP/s even without promotion). A
+//     lane is a token, so a block's scale is one number per thread, and promotion costs one
+//     packed FMA per two values. Two warps per TMEM quadrant, 128 columns each.
+//     Measured, bf16: 4096 x 37888 x 3584 in 477 us (2330 TFLOP/s; 0.50 to 0.56 ms back to back
+//     under the power cap), 1024 x 3584 x 18944 in 69 us, 256 x 3584 x 18944 in 26 us. Bound by
+//     the promotion: 840 cycles a block, where its MMAs take 512.
 //   w8a8_swap_kernel, weight rows as lanes, few tokens: tile of 128 weight rows x 16, 32 or 64
 //     tokens. No tensor-core rows are wasted on missing tokens, the weight stream sets the pace,
 //     and the scale of a column (token) comes from shared memory. One warp per quadrant.
+//     Measured: 16 x 37888 x 3584 in 25.2 us (5.45 TB/s, 85 % of a copy's rate), 16 x 3584 x
+//     18944 in 17.4 us.
 //
-// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue, 2 fetches each block's scales into a
-// small ring, 3 idle; the rest promote. Persistent CTAs (pairs) walk the tiles with the token
-// tile fastest, so the weight tile stays in L2. When there are fewer tiles than SMs, the CTAs of a
-// cluster split K instead and sum their tiles through distributed shared memory in rank order,
-// so the result does not depend on timing and no workspace is needed. Every wait is bounded
-// (2 s): on a time-out the kernel records an error code for tf_device_error, stops, lets its
-// copies and MMAs finish, frees its TMEM and returns. No TMA multicast is used.
+// Warps: 0 TMA producer, 1 TMEM allocation and MMA issue (the pair's warp 3 issues every other
+// block), 2 fetches each block's scales into a small ring; warps from 4 on promote. Persistent CTAs
+// (pairs) walk the tiles with the token tile fastest, so the weight tile stays in L2. When there
+// are fewer tiles than SMs, the CTAs of a cluster split K instead and sum their tiles through
+// distributed shared memory in a fixed order, so the result does not depend on timing and no
+// workspace is needed. Every wait is bounded (2 s): on a time-out the kernel records an error
+// code for tf_device_error, stops, lets its copies and MMAs finish, frees its TMEM and returns. No
+// TMA multicast is used.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 

@@ -7,7 +7,13 @@
 // and feeds their four words to two MMAs: no shared memory, no conversion, no shuffle. The four
 // MMAs of a block start from zero, and their fp32 sum is scaled into the running fp32 sum, so
 // nothing is accumulated across blocks under different scales. K is split over the warps of a
-// CTA (block b goes to warp b mod WK), whose sums are added in warp order in shared memory.
+// CTA (block b goes to warp b mod WK), whose sums are added in warp order in shared memory. More
+// than 8 tokens are more rows of CTAs, which find the weights in L2.
+//
+// Measured: 1 x 3584 x 3584 in 6.0 us with cold weights (4.6 to 5.6 us a call in a stream of them),
+// 64 x 1000 x 1008 in 4.7 us. Bound by launch and one HBM round trip there; on 136 MB it
+// stops at 3.9 TB/s (bytes in flight: 16 warps an SM, three 2 KB blocks each), where the
+// tensor-core kernel takes over.
 #include <algorithm>
 
 #include "tf_common.cuh"
