@@ -35,7 +35,7 @@ __device__ __forceinline__ float4 ld_cluster_v4(uint32_t addr) {
 // Arrival on an mbarrier of any CTA of the cluster (an address from map_to_rank). It tells that
 // this thread's TMEM loads are done and passes no data of other memory, so it is not a release
 // at cluster scope: that form, with its acquiring wait, drains and invalidates L1 on every block
-// (measured: 1.4 us a block, against 0.3).
+// (measured: 1.35 us a block, against 0.73 without).
 __device__ __forceinline__ void mbar_arrive_remote(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
