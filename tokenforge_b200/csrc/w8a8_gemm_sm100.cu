@@ -89,16 +89,28 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, int si
   return mbar_wait_slow(bar, parity, site);
 }
 
-// A wait that nothing ends early: for copies and MMAs in flight, which must finish before shared
-// memory or TMEM is given up.
-__device__ __forceinline__ void mbar_drain(uint64_t* bar, uint32_t parity) {
+// A wait that nothing ends early: for copies and MMAs in flight, and their arrivals, which must
+// finish before shared memory or TMEM is given up. False if it gave up.
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
   const unsigned long long t0 = global_ns();
   while (!mbar_try_wait(bar, parity))
     if (global_ns() - t0 > kWaitLimitNs) {
       atomicCAS(&g_w8a8_error, 0, kErrDrain);
-      return;
+      return false;
     }
+  return true;
 }
+// The commits of a CTA's last blocks arrive on its `empty` barriers asynchronously, and in the pair
+// kernel they come from the other CTA: the producer, whose loads have used stages 0 .. it - 1,
+// waits for those of the last `kStages`, or the CTA could exit, and its shared memory pass to
+// another kernel, with an arrival on the way. After an error some are never sent: one wait then
+// runs into its limit and the others are given up.
+template <int kStages>
+__device__ __forceinline__ void drain_empty(uint64_t* empty, uint32_t it) {
+  for (uint32_t j = it > kStages ? it - kStages : 0; j < it; ++j)
+    if (!mbar_drain(&empty[j % kStages], (j / kStages) & 1u)) return;
+}
+
 // D[tmem] (+)= A[smem] * B[smem]^T, e4m3 inputs, fp32 accumulate, K = 32, issued by one thread
 // (of the leading CTA of a pair).
 __device__ __forceinline__ void umma_e4m3(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc,
@@ -401,6 +413,7 @@ __global__ void __launch_bounds__(Pair::kThreads, 1)
       if (side == 0)
         for (uint32_t j = it > S ? it - S : 0; j < it; ++j)
           mbar_drain(&full[j % S], (j / S) & 1u);
+      drain_empty<S>(empty, it);
     } else if ((warp == 1 || warp == 3) && lane == 0 && side == 0) {
       // Two issuing threads, for even and odd blocks (and TMEM buffers): an MMA's issue waits for
       // the one before it, so while one thread waits on barriers and commits, the other one's
@@ -733,6 +746,7 @@ __global__ void __launch_bounds__(Swap<kCols>::kThreads, 1)
     }
     // Every armed stage must have landed before the CTA may exit.
     for (uint32_t j = it > S ? it - S : 0; j < it; ++j) mbar_drain(&full[j % S], (j / S) & 1u);
+    drain_empty<S>(empty, it);
   } else if (warp == 1 && lane == 0) {
     constexpr uint32_t idesc = idesc_e4m3(kLanes, kCols);
     uint32_t it = 0;
