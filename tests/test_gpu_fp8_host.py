@@ -1,0 +1,39 @@
+"""GPU tests of how the FP8 block-scaled operators behave towards their callers: exception types,
+the interpreter lock, traced programs and errors of earlier launches."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from tokenforge_b200 import ops
+
+pytestmark = pytest.mark.gpu
+E4M3 = torch.float8_e4m3fn
+
+
+def test_outputs_that_do_not_fit_raise_out_of_memory(device: torch.device) -> None:
+    """Under a limit on this process's memory, an output above it raises torch.OutOfMemoryError (a
+    RuntimeError's subclass that serving code catches), from every operator."""
+    x = torch.zeros((1 << 14, 4096), dtype=torch.float16, device=device)
+    w = torch.ones(4096, dtype=torch.float16, device=device)
+    xq = torch.zeros((1 << 14, 16), dtype=E4M3, device=device)
+    xs, ws = torch.ones((1 << 14, 1), device=device), torch.ones((64, 1), device=device)
+    wq = torch.zeros((8192, 16), dtype=E4M3, device=device)
+    calls = [
+        lambda: ops.add_rmsnorm_fp8_quant(x, x, w, 1e-6),
+        lambda: ops.silu_mul_fp8_quant(x),
+        lambda: ops.e4m3_quant_groups(x),
+        lambda: ops.w8a8_block_linear(xq, xs, wq, ws),
+    ]
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(device).total_memory
+    used = torch.cuda.memory_reserved(device)
+    try:
+        torch.cuda.set_per_process_memory_fraction((used + (8 << 20)) / total)
+        for call in calls:
+            with pytest.raises(torch.OutOfMemoryError):
+                call()
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    ops.e4m3_quant_groups(x)

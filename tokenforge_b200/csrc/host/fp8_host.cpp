@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "../../../include/tokenforge_b200.h"
@@ -82,13 +83,14 @@ PyObject* pack(std::initializer_list<Tensor> ts) {
   return tuple;
 }
 
-// Runs `body`, with C++ exceptions turned into Python's.
+// Runs `body`, with C++ exceptions turned into Python's as PyTorch's own bindings do it (an output
+// that does not fit is a torch.OutOfMemoryError).
 template <typename F>
 PyObject* guarded(F body) {
   try {
     return body();
-  } catch (const std::exception& e) {
-    PyErr_SetString(PyExc_RuntimeError, e.what());
+  } catch (...) {
+    torch::translate_exception_to_python(std::current_exception());
     return nullptr;
   }
 }
