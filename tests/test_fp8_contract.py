@@ -213,3 +213,15 @@ def test_abi_activation_status() -> None:
     assert quant(r=-1) == quant(c=0) == quant(ld=7) == quant(dtype=2) == bad
     assert quant(x=None) == quant(q=None) == quant(s=None) == bad
     assert quant(r=0) == _lib.TF_OK
+
+
+# ------------------------------------------------------------------------------- host fast path
+
+
+@pytest.mark.parametrize("group_size", [2**31, -(2**40), 2**70, -(10**30)])
+def test_group_sizes_past_a_machine_word_are_refused(group_size: int) -> None:
+    x = torch.zeros((2, 64), dtype=torch.float16)
+    with pytest.raises(ValueError, match="group_size"):
+        ops.silu_mul_fp8_quant(x, group_size)
+    with pytest.raises(ValueError, match="group_size"):
+        ops.add_rmsnorm_fp8_quant(x, x, x[0], 1e-6, group_size)

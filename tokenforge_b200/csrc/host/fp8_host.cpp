@@ -96,7 +96,8 @@ PyObject* guarded(F body) {
 }
 
 bool group_arg(PyObject* o, int* group) {
-  const long g = PyLong_Check(o) ? PyLong_AsLong(o) : -1;
+  int overflow = 0;  // a number past a long is refused later, like any other wrong one
+  const long g = PyLong_Check(o) ? PyLong_AsLongAndOverflow(o, &overflow) : -1;
   *group = static_cast<int>(g);
   return g == 0 || g == kGroup;
 }
