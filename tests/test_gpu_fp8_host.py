@@ -3,6 +3,9 @@ the interpreter lock, traced programs and errors of earlier launches."""
 
 from __future__ import annotations
 
+import threading
+import time
+
 import pytest
 import torch
 
@@ -37,3 +40,36 @@ def test_outputs_that_do_not_fit_raise_out_of_memory(device: torch.device) -> No
     finally:
         torch.cuda.set_per_process_memory_fraction(1.0)
     ops.e4m3_quant_groups(x)
+
+
+def test_other_threads_run_while_a_launch_waits(device: torch.device) -> None:
+    """With the launch queue full behind a kernel of 0.4 s or more (torch's bounded spin), the call
+    that waits for a free place must let other Python threads run, as every torch call does."""
+    x = torch.zeros((1, 256), dtype=torch.float16, device=device)
+    ops.e4m3_quant_groups(x)
+    gaps: list[float] = []
+    stop = threading.Event()
+
+    def tick() -> None:
+        last = time.perf_counter()
+        while not stop.is_set():
+            time.sleep(0.001)
+            now = time.perf_counter()
+            gaps.append(now - last)
+            last = now
+
+    torch.cuda.synchronize()
+    thread = threading.Thread(target=tick)
+    thread.start()
+    try:
+        begin = time.perf_counter()
+        torch.cuda._sleep(800_000_000)  # cycles: 0.4 s at the highest clock, 1.965 GHz
+        for _ in range(6000):
+            ops.e4m3_quant_groups(x)
+        enqueued = time.perf_counter() - begin
+        torch.cuda.synchronize()
+    finally:
+        stop.set()
+        thread.join()
+    assert enqueued > 0.3, "the queue was not full: nothing waited"
+    assert max(gaps) < 0.15, f"another thread stood still for {max(gaps):.3f} s"

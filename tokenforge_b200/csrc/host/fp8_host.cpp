@@ -95,6 +95,19 @@ PyObject* guarded(F body) {
   }
 }
 
+// The interpreter lock is given up while outputs are allocated and the kernel is launched, either of
+// which may wait (for memory, for a place in the launch queue).
+class Unlocked {
+ public:
+  Unlocked() : state_(PyEval_SaveThread()) {}
+  ~Unlocked() { PyEval_RestoreThread(state_); }
+  Unlocked(const Unlocked&) = delete;
+  Unlocked& operator=(const Unlocked&) = delete;
+
+ private:
+  PyThreadState* state_;
+};
+
 bool group_arg(PyObject* o, int* group) {
   int overflow = 0;  // a number past a long is refused later, like any other wrong one
   const long g = PyLong_Check(o) ? PyLong_AsLongAndOverflow(o, &overflow) : -1;
@@ -122,14 +135,19 @@ PyObject* add_rmsnorm(PyObject*, PyObject* const* args, Py_ssize_t n) {
     if (r && (r->scalar_type() != type || r->sizes() != x->sizes() || !r->is_contiguous()))
       return none();
     const int64_t rows = x->numel() / h, groups = group ? (h + kGroup - 1) / kGroup : 1;
-    Tensor q = empty(x->sizes(), ScalarType::Float8_e4m3fn, device);
-    Tensor scale = empty(with_last(*x, groups), ScalarType::Float, device);
-    Tensor sum = r ? empty(x->sizes(), type, device) : *x;
-    const int st = tf_add_rmsnorm_fp8_quant(
-        ptr<uint16_t>(*x), rows, h, h, r ? ptr<uint16_t>(*r) : nullptr, r ? h : 0,
-        ptr<uint16_t>(*w), static_cast<float>(PyFloat_AS_DOUBLE(args[3])), dtype, group,
-        ptr<uint8_t>(q), ptr<float>(scale), r ? ptr<uint16_t>(sum) : nullptr, h,
-        stream_of(device));
+    const float eps = static_cast<float>(PyFloat_AS_DOUBLE(args[3]));
+    Tensor q, scale, sum;
+    int st;
+    {
+      Unlocked unlocked;
+      q = empty(x->sizes(), ScalarType::Float8_e4m3fn, device);
+      scale = empty(with_last(*x, groups), ScalarType::Float, device);
+      if (r) sum = empty(x->sizes(), type, device);
+      st = tf_add_rmsnorm_fp8_quant(
+          ptr<uint16_t>(*x), rows, h, h, r ? ptr<uint16_t>(*r) : nullptr, r ? h : 0,
+          ptr<uint16_t>(*w), eps, dtype, group, ptr<uint8_t>(q), ptr<float>(scale),
+          r ? ptr<uint16_t>(sum) : nullptr, h, stream_of(device));
+    }
     if (st != TF_OK) return none();
     if (r) return pack({q, scale, sum});
     PyObject* out = pack({q, scale, q});
@@ -155,11 +173,16 @@ PyObject* silu_mul(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t width = x->size(-1);
     if (dtype < 0 || x->numel() == 0 || width % 2 || !x->is_contiguous()) return none();
     const int64_t i = width / 2, rows = x->numel() / width;
-    Tensor q = empty(with_last(*x, i), ScalarType::Float8_e4m3fn, device);
-    Tensor scale = empty(with_last(*x, group ? (i + kGroup - 1) / kGroup : 1), ScalarType::Float,
-                         device);
-    const int st = tf_silu_mul_fp8_quant(ptr<uint16_t>(*x), rows, i, width, dtype, group,
-                                         ptr<uint8_t>(q), ptr<float>(scale), stream_of(device));
+    Tensor q, scale;
+    int st;
+    {
+      Unlocked unlocked;
+      q = empty(with_last(*x, i), ScalarType::Float8_e4m3fn, device);
+      scale = empty(with_last(*x, group ? (i + kGroup - 1) / kGroup : 1), ScalarType::Float,
+                    device);
+      st = tf_silu_mul_fp8_quant(ptr<uint16_t>(*x), rows, i, width, dtype, group, ptr<uint8_t>(q),
+                                 ptr<float>(scale), stream_of(device));
+    }
     return st == TF_OK ? pack({q, scale}) : none();
   });
 }
@@ -174,10 +197,15 @@ PyObject* quant_groups(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int dtype = stream_dtype(x->scalar_type());
     if (dtype < 0 || x->numel() == 0 || !x->is_contiguous()) return none();
     const int64_t c = x->size(-1), rows = x->numel() / c;
-    Tensor q = empty(x->sizes(), ScalarType::Float8_e4m3fn, device);
-    Tensor scale = empty(with_last(*x, (c + kGroup - 1) / kGroup), ScalarType::Float, device);
-    const int st = tf_e4m3_quant_groups(ptr<uint16_t>(*x), rows, c, c, dtype, ptr<uint8_t>(q),
-                                        ptr<float>(scale), stream_of(device));
+    Tensor q, scale;
+    int st;
+    {
+      Unlocked unlocked;
+      q = empty(x->sizes(), ScalarType::Float8_e4m3fn, device);
+      scale = empty(with_last(*x, (c + kGroup - 1) / kGroup), ScalarType::Float, device);
+      st = tf_e4m3_quant_groups(ptr<uint16_t>(*x), rows, c, c, dtype, ptr<uint8_t>(q),
+                                ptr<float>(scale), stream_of(device));
+    }
     return st == TF_OK ? pack({q, scale}) : none();
   });
 }
@@ -211,11 +239,16 @@ PyObject* block_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
               !b->is_contiguous()))
       return none();
     const int64_t m = x->numel() / k;
-    Tensor y = empty(with_last(*x, rows_w), type, device);
-    const int st = tf_w8a8_block_linear(
-        ptr<uint8_t>(*x), m, k, k, ptr<float>(*xs), kb, ptr<uint8_t>(*w), ptr<float>(*ws),
-        b ? ptr<uint16_t>(*b) : nullptr, rows_w, dtype, ptr<uint16_t>(y), rows_w,
-        stream_of(device));
+    Tensor y;
+    int st;
+    {
+      Unlocked unlocked;
+      y = empty(with_last(*x, rows_w), type, device);
+      st = tf_w8a8_block_linear(
+          ptr<uint8_t>(*x), m, k, k, ptr<float>(*xs), kb, ptr<uint8_t>(*w), ptr<float>(*ws),
+          b ? ptr<uint16_t>(*b) : nullptr, rows_w, dtype, ptr<uint16_t>(y), rows_w,
+          stream_of(device));
+    }
     return st == TF_OK ? THPVariable_Wrap(y) : none();
   });
 }
