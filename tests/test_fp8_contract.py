@@ -3,6 +3,8 @@ fakes, the weight bundle, and the C ABI's refusals (each returns before anything
 
 from __future__ import annotations
 
+import warnings
+
 import pytest
 import torch
 
@@ -225,3 +227,61 @@ def test_group_sizes_past_a_machine_word_are_refused(group_size: int) -> None:
         ops.silu_mul_fp8_quant(x, group_size)
     with pytest.raises(ValueError, match="group_size"):
         ops.add_rmsnorm_fp8_quant(x, x, x[0], 1e-6, group_size)
+
+
+@pytest.fixture
+def reload_host_path():  # type: ignore[no-untyped-def]
+    """The host fast path is looked for anew inside the test, and again after it."""
+    from tokenforge_b200 import fp8
+
+    def reset() -> None:
+        fp8._fast = None
+        _lib.fp8_host.cache_clear()
+
+    reset()
+    yield
+    reset()
+
+
+def _careful_path_refuses() -> None:
+    x = torch.zeros((2, 64), dtype=torch.float16)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.e4m3_quant_groups(x)
+    with pytest.raises(ValueError, match="group_size"):
+        ops.silu_mul_fp8_quant(x, 32)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.add_rmsnorm_fp8_quant(x, x, x[0], 1e-6)
+    with pytest.raises(RuntimeError, match="CUDA"):
+        ops.w8a8_block_linear(**_linear_args())
+
+
+def test_an_extension_of_another_pytorch_is_not_loaded(reload_host_path, monkeypatch) -> None:  # type: ignore[no-untyped-def]
+    """The extension holds PyTorch's and CPython's inline code: one built against others is not
+    taken, the operators warn once and go through Python."""
+    monkeypatch.setattr(torch, "__version__", "0.0.1+other")
+    with pytest.warns(RuntimeWarning, match="host fast path"):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            ops.e4m3_quant_groups(torch.zeros((2, 64), dtype=torch.float16))
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        _careful_path_refuses()
+
+
+def test_a_broken_extension_leaves_the_python_path(reload_host_path, monkeypatch, tmp_path) -> None:  # type: ignore[no-untyped-def]
+    broken = tmp_path / "fp8_host.so"
+    broken.write_bytes(b"not a shared object")
+    monkeypatch.setattr(_lib, "host_path", lambda: broken)
+    with pytest.warns(RuntimeWarning, match="host fast path"):
+        _careful_path_refuses()
+
+
+def test_the_build_makes_the_extension_that_is_loaded(reload_host_path) -> None:  # type: ignore[no-untyped-def]
+    import sysconfig
+
+    path = _lib.host_path()
+    assert torch.__version__ in path.name and sysconfig.get_config_var("SOABI") in path.name
+    assert path.exists(), "build() did not make the host extension for this PyTorch"
+    with warnings.catch_warnings():
+        warnings.simplefilter("error")
+        _careful_path_refuses()
+    assert _lib.fp8_host().__file__ == str(path)

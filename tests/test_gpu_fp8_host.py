@@ -10,6 +10,7 @@ import pytest
 import torch
 
 from tokenforge_b200 import ops
+from tokenforge_b200.pack import pack_w8a8_block
 
 pytestmark = pytest.mark.gpu
 E4M3 = torch.float8_e4m3fn
@@ -73,3 +74,22 @@ def test_other_threads_run_while_a_launch_waits(device: torch.device) -> None:
         thread.join()
     assert enqueued > 0.3, "the queue was not full: nothing waited"
     assert max(gaps) < 0.15, f"another thread stood still for {max(gaps):.3f} s"
+
+
+def test_without_the_extension_the_results_are_the_same(device: torch.device, monkeypatch) -> None:  # type: ignore[no-untyped-def]
+    from tokenforge_b200 import fp8
+
+    gen = torch.Generator(device=device).manual_seed(5)
+    x = torch.randn((20, 640), generator=gen, device=device).bfloat16()
+    p = pack_w8a8_block(torch.randn((200, 640), generator=gen, device=device))
+    w = torch.ones(640, dtype=torch.bfloat16, device=device)
+
+    def run():  # type: ignore[no-untyped-def]
+        q, s, h = ops.add_rmsnorm_fp8_quant(x, x, w, 1e-6)
+        y = ops.w8a8_block_linear(q, s, p.wq, p.w_scale, None, torch.bfloat16)
+        return [q, s, h, y, *ops.silu_mul_fp8_quant(x, 0), *ops.e4m3_quant_groups(x)]
+
+    want = run()
+    monkeypatch.setattr(fp8, "_fast", fp8._NoFastPath())
+    for a, b in zip(want, run(), strict=True):
+        assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))

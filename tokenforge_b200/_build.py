@@ -5,8 +5,9 @@ arch=compute_100a,code=sm_100a``) into ``_build/`` and linked into one shared li
 CUDA runtime linked statically, so the library has no dependency beyond the driver. The C ABI
 it exports is declared in ``include/tokenforge_b200.h``.
 
-Beside it, ``lib/fp8_host.so`` is the host fast path of the FP8 operators (``csrc/host``), a
-CPython extension compiled by the host compiler against PyTorch's headers.
+Beside it, ``lib/fp8_host.*.so`` is the host fast path of the FP8 operators (``csrc/host``), a
+CPython extension compiled by the host compiler against PyTorch's headers (a file for each PyTorch
+and CPython it is built against).
 
     python -m tokenforge_b200._build [--force] [--verbose]
 """
@@ -28,7 +29,6 @@ CSRC = PKG / "csrc"
 BUILD = PKG / "_build"
 LIB = PKG / "lib" / "libtokenforge_b200.so"
 HOST_SRC = CSRC / "host" / "fp8_host.cpp"
-HOST_LIB = PKG / "lib" / "fp8_host.so"
 INCLUDE = ROOT / "include"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -86,16 +86,19 @@ def _compile(src: Path, verbose: bool) -> Path:
 
 def _build_host(force: bool) -> None:
     """The CPython extension: linked against PyTorch and the kernel library next to it."""
-    if not force and not _stale(HOST_LIB, [HOST_SRC, LIB, *INCLUDE.glob("*.h")]):
-        return
     import torch
 
+    from tokenforge_b200 import _lib
+
+    target = _lib.host_path()
+    if not force and not _stale(target, [HOST_SRC, LIB, *INCLUDE.glob("*.h")]):
+        return
     cxx = os.environ.get("CXX") or shutil.which("g++") or shutil.which("c++")
     if cxx is None:
         raise RuntimeError("g++ not found: a C++ compiler is required to build tokenforge_b200")
     pt = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
-    tmp = HOST_LIB.with_suffix(".so.tmp")
+    tmp = target.with_suffix(".so.tmp")
     cmd = [
         cxx, "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
         f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
@@ -108,7 +111,7 @@ def _build_host(force: bool) -> None:
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"{cxx} failed on {HOST_SRC.name}:\n{proc.stderr}")
-    os.replace(tmp, HOST_LIB)
+    os.replace(tmp, target)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:

@@ -10,13 +10,21 @@ import ctypes
 import functools
 import importlib.machinery
 import importlib.util
+import sysconfig
 import threading
 from pathlib import Path
 
 import torch
 
 LIB_PATH = Path(__file__).resolve().parent / "lib" / "libtokenforge_b200.so"
-HOST_PATH = LIB_PATH.with_name("fp8_host.so")
+
+
+def host_path() -> Path:
+    """The host extension's file. It holds inline code of PyTorch and CPython, so its name says
+    which of them it was built against: with others it is another file, to be built anew."""
+    build = f"{torch.__version__}-{(torch.version.git_version or '')[:8]}"
+    return LIB_PATH.with_name(f"fp8_host.{sysconfig.get_config_var('SOABI')}.torch-{build}.so")
+
 
 TF_OK = 0
 TF_ERR_INVALID_ARG = 1
@@ -191,13 +199,14 @@ def lib() -> ctypes.CDLL:
 def fp8_host():  # type: ignore[no-untyped-def]
     """The host fast path of the FP8 operators (``csrc/host/fp8_host.cpp``)."""
     lib()  # the kernel library it is linked against, with its own message if it is missing
-    if not HOST_PATH.exists():
+    path = host_path()
+    if not path.exists():
         raise ImportError(
-            f"tokenforge_b200 host extension not found at {HOST_PATH}; build it with "
+            f"tokenforge_b200 host extension not found at {path}; build it with "
             "`python -m tokenforge_b200._build`"
         )
-    loader = importlib.machinery.ExtensionFileLoader("fp8_host", str(HOST_PATH))
-    spec = importlib.util.spec_from_file_location("fp8_host", str(HOST_PATH), loader=loader)
+    loader = importlib.machinery.ExtensionFileLoader("fp8_host", str(path))
+    spec = importlib.util.spec_from_file_location("fp8_host", str(path), loader=loader)
     module = importlib.util.module_from_spec(spec)
     loader.exec_module(module)
     return module
