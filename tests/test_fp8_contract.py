@@ -285,3 +285,16 @@ def test_the_build_makes_the_extension_that_is_loaded(reload_host_path) -> None:
         warnings.simplefilter("error")
         _careful_path_refuses()
     assert _lib.fp8_host().__file__ == str(path)
+
+
+def test_registered_norm_without_a_residual_returns_packed_rows(monkeypatch) -> None:  # type: ignore[no-untyped-def]
+    """The copy of x that the registered operator returns has the fake's layout, not x's own. The
+    kernel's part is stood in for, so that the wrapper runs without a GPU."""
+    def launcher(x, residual, weight, eps, group_size):  # type: ignore[no-untyped-def]
+        return torch.empty(x.shape, dtype=E4M3), torch.empty((*x.shape[:-1], 1)), x
+
+    monkeypatch.setattr(ops, "add_rmsnorm_fp8_quant", launcher)
+    x = torch.randn((4, 3, 64)).half().transpose(0, 1)
+    h = torch.ops.tokenforge.add_rmsnorm_fp8_quant(x, None, x[0, 0], 1e-6, 0)[2]
+    assert torch.equal(h, x) and h.data_ptr() != x.data_ptr()
+    assert h.stride() == (256, 64, 1)

@@ -93,3 +93,45 @@ def test_without_the_extension_the_results_are_the_same(device: torch.device, mo
     monkeypatch.setattr(fp8, "_fast", fp8._NoFastPath())
     for a, b in zip(want, run(), strict=True):
         assert a.dtype == b.dtype and torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+def _operands(device):  # type: ignore[no-untyped-def]
+    """Arguments of the four registered operators on inputs of several layouts."""
+    gen = torch.Generator(device=device).manual_seed(3)
+    w = torch.ones(64, dtype=torch.float16, device=device)
+    p = pack_w8a8_block(torch.randn((48, 64), generator=gen, device=device))
+
+    def layouts(c):  # type: ignore[no-untyped-def]
+        base = torch.randn((4, 3, 2 * c), generator=gen, device=device).half()
+        return [base[:, :, :c].contiguous(), base[:, :, :c], base[:, :, :c].contiguous().transpose(0, 1),
+                base[:, :, ::2], base[:, :, :c].contiguous().permute(2, 0, 1).contiguous().permute(1, 2, 0)]
+
+    t = torch.ops.tokenforge
+    for x in layouts(64):
+        yield t.add_rmsnorm_fp8_quant, (x, None, w, 1e-6, 128)
+        yield t.add_rmsnorm_fp8_quant, (x, x.flip(0), w, 1e-6, 0)
+        yield t.silu_mul_fp8_quant, (x, 128)
+        yield t.e4m3_quant_groups, (x,)
+        q, s = ops.e4m3_quant_groups(x)
+        yield t.w8a8_block_linear, (q, s, p.wq, p.w_scale, None, torch.bfloat16)
+        q, s = q.transpose(0, 1), s.transpose(0, 1)
+        yield t.w8a8_block_linear, (q, s, p.wq, p.w_scale, None, torch.float16)
+
+
+def test_registered_ops_pass_opcheck(device: torch.device) -> None:
+    """test_schema multiplies its inputs and outputs, which torch does not do in e4m3."""
+    for op, args in _operands(device):
+        torch.library.opcheck(op.default, args, test_utils="test_faketensor")
+
+
+def test_fakes_give_the_strides(device: torch.device) -> None:
+    """What a traced program plans with is what the operator returns, layout included."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    for op, args in _operands(device):
+        real = op(*args)
+        with FakeTensorMode() as mode:
+            fake = op(*[mode.from_tensor(a) if isinstance(a, torch.Tensor) else a for a in args])
+        real, fake = (r if isinstance(r, tuple) else (r,) for r in (real, fake))
+        for r, f in zip(real, fake, strict=True):
+            assert (r.shape, r.dtype, r.stride()) == (f.shape, f.dtype, f.stride()), (op, args)

@@ -525,7 +525,8 @@ def e4m3_quant_rows(y: torch.Tensor, scale: torch.Tensor | None = None
 #
 # tokenforge_b200.fp8 holds the launchers, exported here for direct calls; the registrations
 # below give the same operators to traced programs (a custom op may not return its input, so
-# without a residual the registered norm returns a copy of x).
+# without a residual the registered norm returns a copy of x, packed like every other output and
+# like the fake's whatever the layout of x).
 
 
 @torch.library.custom_op("tokenforge::w8a8_block_linear", mutates_args=())
@@ -554,7 +555,9 @@ def _add_rmsnorm_fp8_quant_op(
     group_size: int,
 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     q, s, total = add_rmsnorm_fp8_quant(x, residual, weight, eps, group_size)
-    return q, s, total.clone() if residual is None else total
+    if residual is None:
+        total = total.clone(memory_format=torch.contiguous_format)
+    return q, s, total
 
 
 def _group_scales(x, columns, group_size):  # type: ignore[no-untyped-def]
