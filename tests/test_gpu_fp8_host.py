@@ -9,7 +9,7 @@ import time
 import pytest
 import torch
 
-from tokenforge_b200 import ops
+from tokenforge_b200 import _lib, ops
 from tokenforge_b200.pack import pack_w8a8_block
 
 pytestmark = pytest.mark.gpu
@@ -135,3 +135,57 @@ def test_fakes_give_the_strides(device: torch.device) -> None:
         real, fake = (r if isinstance(r, tuple) else (r,) for r in (real, fake))
         for r, f in zip(real, fake, strict=True):
             assert (r.shape, r.dtype, r.stride()) == (f.shape, f.dtype, f.stride()), (op, args)
+
+
+def _launches(lib, device):  # type: ignore[no-untyped-def]
+    """C ABI calls of every FP8 kernel's launcher, each taking a stream."""
+    x = torch.zeros((600, 512), dtype=torch.float16, device=device)
+    w = torch.ones(512, dtype=torch.float16, device=device)
+    q = torch.zeros((600, 512), dtype=torch.uint8, device=device)
+    s = torch.zeros((600, 4), device=device)
+    wq = torch.zeros((512, 512), dtype=torch.uint8, device=device)
+    ws = torch.zeros((4, 4), device=device)
+    h, y = torch.empty_like(x), torch.empty_like(x)
+
+    def linear(m, n):  # type: ignore[no-untyped-def]
+        return lambda stream: lib.tf_w8a8_block_linear(
+            q.data_ptr(), m, 512, 512, s.data_ptr(), 4, wq.data_ptr(), ws.data_ptr(), None, n, 0,
+            y.data_ptr(), 512, stream)
+
+    return {
+        "quant": lambda stream: lib.tf_e4m3_quant_groups(
+            x.data_ptr(), 4, 512, 512, 0, q.data_ptr(), s.data_ptr(), stream),
+        "silu": lambda stream: lib.tf_silu_mul_fp8_quant(
+            x.data_ptr(), 4, 256, 512, 0, 0, q.data_ptr(), s.data_ptr(), stream),
+        "norm": lambda stream: lib.tf_add_rmsnorm_fp8_quant(
+            x.data_ptr(), 4, 512, 512, x.data_ptr(), 512, w.data_ptr(), 1e-6, 0, 128,
+            q.data_ptr(), s.data_ptr(), h.data_ptr(), 512, stream),
+        "linear, warp MMA": linear(4, 512),
+        "linear, tensor cores": linear(600, 512),
+    }
+
+
+@pytest.mark.parametrize("name", ["quant", "silu", "norm", "linear, warp MMA",
+                                  "linear, tensor cores"])
+def test_a_refused_launch_does_not_fail_the_next_call(name: str, device: torch.device) -> None:
+    """A launch that CUDA refuses (here: into the legacy stream while another stream captures) is
+    reported by its own call alone; the next calls of the library succeed."""
+    from cuda.bindings import runtime as rt
+
+    lib = _lib.lib()
+    launch = _launches(lib, device)[name]
+    words = torch.zeros((128, 2), dtype=torch.int32, device=device)
+    packed = torch.zeros((16, 16), dtype=torch.int32, device=device)
+    torch.cuda.synchronize()
+    err, side = rt.cudaStreamCreate()  # a blocking one: it excludes work in the legacy stream
+    assert err == 0
+    mode = rt.cudaStreamCaptureMode.cudaStreamCaptureModeGlobal
+    assert rt.cudaStreamBeginCapture(side, mode)[0] == 0
+    status = launch(None)
+    rt.cudaStreamEndCapture(side)
+    rt.cudaStreamDestroy(side)
+    assert status == _lib.TF_ERR_CUDA
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.tf_awq_repack(words.data_ptr(), 128, 16, packed.data_ptr(), stream) == _lib.TF_OK
+    assert launch(stream) == _lib.TF_OK
+    torch.cuda.synchronize()

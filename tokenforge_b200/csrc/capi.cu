@@ -282,20 +282,14 @@ void* g_noalloc_ptr[kMaxDevices] = {};
 int noalloc_scratch(void** out) {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   if (dev < 0 || dev >= kMaxDevices) return TF_ERR_UNSUPPORTED;
   std::lock_guard<std::mutex> lock(g_noalloc_mu);
   if (g_noalloc_ptr[dev] == nullptr) {
     void* p = nullptr;
     e = cudaGetSymbolAddress(&p, g_noalloc_scratch);
     if (e != cudaSuccess || p == nullptr) {
-      cudaGetLastError();
-      last_cuda_error() = static_cast<int>(e);
-      return TF_ERR_CUDA;
+      return cuda_failed(e);
     }
     g_noalloc_ptr[dev] = p;
   }
@@ -408,9 +402,7 @@ int tf_peer_mailbox_alloc(size_t bytes, void** mailbox, void* ipc_handle) {
   if (e == cudaSuccess) e = cudaIpcGetMemHandle(&h, p);
   if (e != cudaSuccess) {
     if (p) cudaFree(p);
-    tfb::last_cuda_error() = static_cast<int>(e);
-    cudaGetLastError();
-    return TF_ERR_CUDA;
+    return tfb::cuda_failed(e);
   }
   std::memcpy(ipc_handle, &h, sizeof(h));
   *mailbox = p;
@@ -422,33 +414,21 @@ int tf_peer_mailbox_open(const void* ipc_handle, void** mailbox) {
   cudaIpcMemHandle_t h;
   std::memcpy(&h, ipc_handle, sizeof(h));
   const cudaError_t e = cudaIpcOpenMemHandle(mailbox, h, cudaIpcMemLazyEnablePeerAccess);
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    cudaGetLastError();
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   return TF_OK;
 }
 
 int tf_peer_mailbox_close(void* peer_mailbox) {
   if (!peer_mailbox) return TF_ERR_INVALID_ARG;
   const cudaError_t e = cudaIpcCloseMemHandle(peer_mailbox);
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    cudaGetLastError();
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   return TF_OK;
 }
 
 int tf_peer_mailbox_free(void* mailbox) {
   if (!mailbox) return TF_ERR_INVALID_ARG;
   const cudaError_t e = cudaFree(mailbox);
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    cudaGetLastError();
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   return TF_OK;
 }
 
@@ -458,11 +438,7 @@ int tf_peer_mailbox_error(void* mailbox, int* out_code) {
   uint32_t v = 0;
   cudaError_t e = cudaMemcpy(&v, err, sizeof(v), cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && v != 0) e = cudaMemset(err, 0, sizeof(v));
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    cudaGetLastError();
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   *out_code = static_cast<int>(v);
   return TF_OK;
 }

@@ -505,10 +505,7 @@ int launch(void (*kernel)(Args...), int64_t grid, int threads, cudaStream_t stre
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a...);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 

@@ -509,10 +509,7 @@ int launch_rows(void (*kern)(KArgs...), unsigned grid, unsigned threads, cudaStr
   cfg.attrs = attr;
   cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return check_launch();
 }
 
@@ -536,10 +533,7 @@ int launch_stream(const RmsStream& p0, cudaStream_t stream) {
     const cudaError_t e = cudaFuncSetAttribute(rmsnorm_fp8_stream_kernel<VPL>,
                                                cudaFuncAttributeMaxDynamicSharedMemorySize,
                                                kSmemLimit);
-    if (e != cudaSuccess) {
-      last_cuda_error() = static_cast<int>(e);
-      return TF_ERR_CUDA;
-    }
+    if (e != cudaSuccess) return cuda_failed(e);
     if (dev < 64) attr_set.fetch_or(uint64_t{1} << dev);
   }
   const int64_t grid = std::min<int64_t>(device_sms(), cdiv(p.T, nw));
@@ -554,10 +548,7 @@ int launch_stream(const RmsStream& p0, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, rmsnorm_fp8_stream_kernel<VPL>, p);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return check_launch();
 }
 
@@ -565,20 +556,14 @@ int launch_stream(const RmsStream& p0, cudaStream_t stream) {
 
 int rms_device_error(int* code) {
   const cudaError_t e = cudaMemcpyFromSymbol(code, g_rms_error, sizeof(int));
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 
 int rms_reset_device_error() {
   const int zero = 0;
   const cudaError_t e = cudaMemcpyToSymbol(g_rms_error, &zero, sizeof(int));
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 

@@ -12,13 +12,17 @@ namespace tfb {
 // Host-side record of the last CUDA error (per thread), surfaced by tf_last_cuda_error().
 int& last_cuda_error();
 
+// The status of a CUDA call that failed with `e`. Taken off the runtime's own record too, where the
+// check_launch of the next, good, call would find it.
+inline int cuda_failed(cudaError_t e) {
+  last_cuda_error() = static_cast<int>(e);
+  cudaGetLastError();
+  return TF_ERR_CUDA;
+}
+
 inline int check_launch() {
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
-  return TF_OK;
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TF_OK : cuda_failed(e);
 }
 
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -656,11 +656,7 @@ int tf_decode_chain_create(const TfChainOp* ops, int32_t n_ops, int64_t M, int32
   int sms = 0, coop = 0;
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   if (e == cudaSuccess) e = cudaDeviceGetAttribute(&coop, cudaDevAttrCooperativeLaunch, dev);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   if (!coop) return TF_ERR_UNSUPPORTED;
   ChainPlan pl;
   int st = plan_chain(ns.data(), ks.data(), n_ops, static_cast<int>(M), sms, &pl);
@@ -780,11 +776,7 @@ int tf_decode_chain_run(TfChain* chain, void* stream) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, tfb::w4a16_chain_kernel, chain->params);
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    tfb::last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   return TF_OK;
 }
 
@@ -794,11 +786,7 @@ int tf_decode_chain_error(TfChain* chain, int* out_code) {
   uint32_t* err = chain->params.ctl + 2;
   cudaError_t e = cudaMemcpy(&v, err, sizeof(v), cudaMemcpyDeviceToHost);
   if (e == cudaSuccess && v != 0) e = cudaMemset(err, 0, sizeof(v));
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    tfb::last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   *out_code = static_cast<int>(v);
   return TF_OK;
 }
@@ -808,11 +796,7 @@ int tf_decode_chain_destroy(TfChain* chain) {
   cudaError_t e = cudaSuccess;
   if (chain->mem) e = cudaFree(chain->mem);
   delete chain;
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    tfb::last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   return TF_OK;
 }
 

@@ -611,10 +611,7 @@ int launch_bm(const LinearPlan& pl, const LinearArgs& a, cudaStream_t stream) {
     p.tickets = reinterpret_cast<uint32_t*>(static_cast<char*>(a.workspace) + partial);
     const cudaError_t me = cudaMemsetAsync(p.tickets, 0, static_cast<size_t>(p.units) * 4 *
                                                              sizeof(uint32_t), stream);
-    if (me != cudaSuccess) {
-      last_cuda_error() = static_cast<int>(me);
-      return TF_ERR_CUDA;
-    }
+    if (me != cudaSuccess) return cuda_failed(me);
   }
 
   static std::once_flag attr_once[64];
@@ -625,10 +622,7 @@ int launch_bm(const LinearPlan& pl, const LinearArgs& a, cudaStream_t stream) {
     attr_err = cudaFuncSetAttribute(w4a16_tc_kernel<BM, KB>,
                                     cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmemBytes);
   });
-  if (attr_err != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(attr_err);
-    return TF_ERR_CUDA;
-  }
+  if (attr_err != cudaSuccess) return cuda_failed(attr_err);
 
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(pl.stream_k ? pl.grid_x : static_cast<unsigned>(std::min(p.units, num_sms())));
@@ -641,10 +635,7 @@ int launch_bm(const LinearPlan& pl, const LinearArgs& a, cudaStream_t stream) {
   cfg.attrs = attr;
   cfg.numAttrs = (launch_flags() & TF_LAUNCH_PDL) ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, w4a16_tc_kernel<BM, KB>, mx, mw, ms, mz, p);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   if (pl.split_k == 1) return TF_OK;
   return launch_splitk_reduce(p.partial, pl.split_k, a.M, a.N, a.bias, a.y, a.ldy, stream);
 }
@@ -740,10 +731,7 @@ int launch_tc_gemm(const LinearPlan& pl, const LinearArgs& a, cudaStream_t strea
 extern "C" int tf_device_error(int* out_code) {
   if (!out_code) return TF_ERR_INVALID_ARG;
   const cudaError_t e = cudaMemcpyFromSymbol(out_code, tfb::g_device_error, sizeof(int));
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   if (*out_code != 0) return TF_OK;
   const int st = tfb::rms_device_error(out_code);
   return st != TF_OK || *out_code != 0 ? st : tfb::w8a8_device_error(out_code);
@@ -752,10 +740,7 @@ extern "C" int tf_device_error(int* out_code) {
 extern "C" int tf_reset_device_error(void) {
   const int zero = 0;
   const cudaError_t e = cudaMemcpyToSymbol(tfb::g_device_error, &zero, sizeof(int));
-  if (e != cudaSuccess) {
-    tfb::last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return tfb::cuda_failed(e);
   const int st = tfb::rms_reset_device_error();
   return st != TF_OK ? st : tfb::w8a8_reset_device_error();
 }

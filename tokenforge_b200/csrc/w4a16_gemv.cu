@@ -802,10 +802,7 @@ int launch_gemv_grid(Kernel kern, const LinearPlan& plan, const GemvParams& p, s
   if (smem + static_smem > 48 * 1024) {
     const cudaError_t e =
         cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
-    if (e != cudaSuccess) {
-      last_cuda_error() = static_cast<int>(e);
-      return TF_ERR_CUDA;
-    }
+    if (e != cudaSuccess) return cuda_failed(e);
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(plan.grid_x, plan.grid_y, 1);
@@ -829,10 +826,7 @@ int launch_gemv_grid(Kernel kern, const LinearPlan& plan, const GemvParams& p, s
   cfg.attrs = attr;
   cfg.numAttrs = na;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kern, p);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 

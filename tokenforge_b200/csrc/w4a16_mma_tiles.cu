@@ -325,10 +325,7 @@ int launch_variant(const LinearPlan& plan, const MmaParams& p, cudaStream_t stre
   cfg.attrs = attr;
   cfg.numAttrs = pdl ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, w4a16_mma_kernel<MT, WN, WK>, p);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 

@@ -969,11 +969,7 @@ int tc_prepare(TcDevice& d, TcKernel kernel, int threads, int smem, int base) {
         tc_config(static_cast<unsigned>(c), threads, smem, c, nullptr, attr);
     e = cudaOccupancyMaxActiveClusters(&d.clusters[c], kernel, &cfg);
   }
-  if (e != cudaSuccess) {
-    cudaGetLastError();
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   d.ready.store(1, std::memory_order_release);
   return TF_OK;
 }
@@ -1012,10 +1008,7 @@ int tc_launch(const TcDevice& d, TcKernel kernel, int threads, int smem, int bas
       tc_config(static_cast<unsigned>(clusters * base * p.splits), threads, smem,
                 base * p.splits, stream, attr);
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps[0], maps[1], maps[2], p);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 
@@ -1035,10 +1028,7 @@ constexpr int kMaxDevices = 64;
 
 int current_device(int* dev) {
   const cudaError_t e = cudaGetDevice(dev);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return *dev < kMaxDevices ? TF_OK : TF_ERR_UNSUPPORTED;
 }
 
@@ -1156,20 +1146,14 @@ int launch_w8a8_tc(const W8A8Args& a, cudaStream_t stream) {
 
 int w8a8_device_error(int* code) {
   const cudaError_t e = cudaMemcpyFromSymbol(code, g_w8a8_error, sizeof(int));
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 
 int w8a8_reset_device_error() {
   const int zero = 0;
   const cudaError_t e = cudaMemcpyToSymbol(g_w8a8_error, &zero, sizeof(int));
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 

@@ -164,10 +164,7 @@ int launch_w8a8_gemv(const W8A8Args& a, cudaStream_t stream) {
                             ? cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__half>, a, wk, w_early)
                             : cudaLaunchKernelEx(&cfg, w8a8_gemv_kernel<__nv_bfloat16>, a, wk,
                                                  w_early);
-  if (e != cudaSuccess) {
-    last_cuda_error() = static_cast<int>(e);
-    return TF_ERR_CUDA;
-  }
+  if (e != cudaSuccess) return cuda_failed(e);
   return TF_OK;
 }
 
