@@ -12,8 +12,18 @@ from __future__ import annotations
 import pytest
 import torch
 
-from tests.test_gpu_fp8_block import _linear_inputs
+from tests.test_gpu_fp8_block import (
+    DELTA,
+    DTYPES,
+    EPS,
+    _check_codes,
+    _check_linear,
+    _gen,
+    _linear_inputs,
+    _stream,
+)
 from tokenforge_b200 import _lib, ops
+from tokenforge_b200.pack import pack_w8a8_block
 
 pytestmark = pytest.mark.gpu
 
@@ -36,3 +46,202 @@ def test_tensor_core_kernels_back_to_back(device: torch.device) -> None:
     for size, g, w in zip(sizes, got, want):
         assert torch.equal(g, w), size
     assert _lib.device_error() == 0
+
+
+# (n, k) by the number of tokens: the widths reach the kernel named, for pairs with K split over a
+# cluster and not, with output rows of whole 16-byte vectors and not, one and several tiles a pair.
+FORMS = [
+    pytest.param(12, 2050, 2576, id="16 columns"),
+    pytest.param(24, 3600, 2576, id="32 columns"),
+    pytest.param(48, 2000, 4112, id="64 columns"),
+    pytest.param(640, 264, 2576, id="pairs, split"),
+    pytest.param(600, 1003, 4112, id="pairs, split, odd rows"),
+    pytest.param(2560, 4608, 400, id="pairs, several tiles"),
+    pytest.param(2049, 4613, 400, id="pairs, several tiles, odd rows"),
+]
+
+
+@pytest.mark.parametrize("m, n, k", FORMS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("bias", [False, True])
+def test_linear_of_each_form(m: int, n: int, k: int, dtype: torch.dtype, bias: bool,
+                             device: torch.device) -> None:
+    args = _linear_inputs(m, n, k, dtype, bias, device)
+    y = ops.w8a8_block_linear(*args, dtype)
+    _check_linear(y, *args)
+    assert torch.equal(y, ops.w8a8_block_linear(*args, dtype)), "a second call differs"
+
+
+@pytest.mark.parametrize("m, n, k", FORMS)
+def test_special_values_in_each_form(m: int, n: int, k: int, device: torch.device) -> None:
+    """A NaN code or scale reaches its own row (or column, or 128 columns) alone; zero scales give
+    0; an overflowing sum gives the output type's infinity."""
+    xq, xs, wq, ws, _ = _linear_inputs(m, n, k, torch.float16, False, device)
+    row, col = m - 2, n // 2 + 1
+    x2, w2 = xq.clone().view(torch.uint8), wq.clone().view(torch.uint8)
+    x2[row, 130] = 0x7F
+    nan = torch.isnan(ops.w8a8_block_linear(x2, xs, wq, ws))
+    assert bool(nan[row].all()) and int(nan.sum()) == n
+    w2[col, 300] = 0xFF
+    nan = torch.isnan(ops.w8a8_block_linear(xq, xs, w2, ws))
+    assert bool(nan[:, col].all()) and int(nan.sum()) == m
+    xs2, ws2 = xs.clone(), ws.clone()
+    xs2[row, -1] = float("nan")
+    nan = torch.isnan(ops.w8a8_block_linear(xq, xs2, wq, ws))
+    assert bool(nan[row].all()) and int(nan.sum()) == n
+    ws2[col // 128, 1] = float("nan")
+    nan = torch.isnan(ops.w8a8_block_linear(xq, xs, wq, ws2))
+    lo, hi = col // 128 * 128, min(n, col // 128 * 128 + 128)
+    assert bool(nan[:, lo:hi].all()) and int(nan.sum()) == m * (hi - lo)
+    assert not bool(ops.w8a8_block_linear(xq, torch.zeros_like(xs), wq, ws).any())
+    big = torch.full((m, k), 448.0, device=device).to(torch.float8_e4m3fn)
+    y = ops.w8a8_block_linear(big, torch.ones_like(xs), big[:1].repeat(n, 1), torch.ones_like(ws))
+    assert bool(torch.isposinf(y).all())
+
+
+@pytest.mark.parametrize("m, n, k", FORMS)
+@pytest.mark.parametrize("extra", [8, 13])
+def test_each_form_writes_its_rows_only(m: int, n: int, k: int, extra: int,
+                                        device: torch.device) -> None:
+    """C ABI with an output wider than N and rows behind the last token."""
+    xq, xs, wq, ws, _ = _linear_inputs(m, n, k, torch.float16, False, device)
+    y = torch.full((m + 300, n + extra), 7.0, dtype=torch.float16, device=device)
+    status = _lib.lib().tf_w8a8_block_linear(
+        xq.data_ptr(), m, k, k, xs.data_ptr(), xs.shape[1], wq.data_ptr(), ws.data_ptr(), None, n,
+        _lib.TF_DTYPE_FP16, y.data_ptr(), n + extra, _lib.stream_ptr(torch.device("cuda", 0)))
+    _lib.check("tf_w8a8_block_linear", status)
+    _check_linear(y[:m, :n], xq, xs, wq, ws, None)
+    assert bool((y[m:] == 7).all()) and bool((y[:, n:] == 7).all())
+
+
+def test_threads_through_each_form(device: torch.device) -> None:
+    """Four host threads, a stream each, through every form of the linear at once."""
+    import threading
+
+    args = [_linear_inputs(*f.values, torch.bfloat16, True, device) for f in FORMS]
+    want = [ops.w8a8_block_linear(*a, torch.bfloat16) for a in args]
+    torch.cuda.synchronize()
+    same = []
+
+    def work() -> None:
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            for _ in range(10):
+                got = [ops.w8a8_block_linear(*a, torch.bfloat16) for a in args]
+            stream.synchronize()
+            same.append(all(torch.equal(a, b) for a, b in zip(got, want)))
+
+    threads = [threading.Thread(target=work) for _ in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert same == [True] * 4
+    assert _lib.device_error() == 0
+
+
+@pytest.mark.parametrize("m", [24, 700])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mlp_block_through_the_tensor_cores(m: int, dtype: torch.dtype,
+                                            device: torch.device) -> None:
+    """The MLP half of a decoder layer at sizes whose linears are the 32-column kernel and the CTA
+    pairs: each step against its definition on the step's inputs, then captured and replayed on new
+    ones, and with programmatic dependent launch."""
+    h, i = 1280, 2368
+    gen = _gen(m, 17)
+    w1 = pack_w8a8_block(torch.randn((2 * i, h), generator=gen, device=device) / h**0.5)
+    w2 = pack_w8a8_block(torch.randn((4 * h, i), generator=gen, device=device) / i**0.5)
+    gamma = (1 + 0.1 * torch.randn(h, generator=gen, device=device)).to(dtype)
+    gamma4 = (1 + 0.1 * torch.randn(4 * h, generator=gen, device=device)).to(dtype)
+    x, r = _stream(m, h, dtype, 12, device, 1.0), _stream(m, h, dtype, 13, device, 3.0)
+
+    def run(check: bool):  # type: ignore[no-untyped-def]
+        q, s, _ = ops.add_rmsnorm_fp8_quant(x, r, gamma, EPS)
+        gu = ops.w8a8_block_linear(q, s, w1.wq, w1.w_scale, None, dtype)
+        q2, s2 = ops.silu_mul_fp8_quant(gu)
+        d = ops.w8a8_block_linear(q2, s2, w2.wq, w2.w_scale, None, dtype)
+        q3, s3, total = ops.add_rmsnorm_fp8_quant(d, d, gamma4, EPS, 0)
+        if check:
+            _check_linear(gu, q, s, w1.wq, w1.w_scale, None)
+            _check_linear(d, q2, s2, w2.wq, w2.w_scale, None)
+            a, b = gu.double().chunk(2, 1)
+            _check_codes(q2, s2, a / (1 + torch.exp(-a)) * b, 128, DELTA["silu"])
+            f = total.double()
+            y64 = f / torch.sqrt(f.square().mean(1, keepdim=True) + EPS) * gamma4.double()
+            _check_codes(q3, s3, y64, 0, DELTA["norm"])
+        return q3, s3, total
+
+    def same(a, b):  # type: ignore[no-untyped-def]
+        return all(torch.equal(u.view(torch.uint8), v.view(torch.uint8)) for u, v in zip(a, b))
+
+    want = run(True)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run(False)
+    graph.replay()
+    assert same(got, want)
+    x.copy_(x.flip(1))
+    want = run(True)
+    graph.replay()
+    assert same(got, want)
+    old = _lib.get_launch_flags()
+    try:
+        _lib.set_launch_flags(_lib.TF_LAUNCH_PDL)
+        for _ in range(20):
+            last = run(False)
+        assert same(last, want)
+    finally:
+        _lib.set_launch_flags(old)
+
+
+# ------------------------------------------------------------------- rows beyond the first pass
+
+# More rows than the launch has CTAs (148 SMs times the resident CTAs of each width), so that every
+# CTA walks several: 1, 2, 4 and 8 vectors a thread.
+LONG = [(10001, 256), (1300, 3584), (500, 8200), (400, 18944)]
+
+
+def _norm64(total, w):  # type: ignore[no-untyped-def]
+    f = total.double()
+    return f / torch.sqrt(f.square().mean(1, keepdim=True) + EPS) * w.double()
+
+
+@pytest.mark.parametrize("t, h", LONG)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("group", [128, 0])
+def test_norm_of_many_rows(t: int, h: int, dtype: torch.dtype, group: int,
+                           device: torch.device) -> None:
+    x, r = _stream(t, h, dtype, 1, device, 1.0), _stream(t, h, dtype, 2, device, 4.0)
+    w = (1 + 0.1 * torch.randn(h, generator=_gen(h), device=device)).to(dtype)
+    q, s, total = ops.add_rmsnorm_fp8_quant(x, r, w, EPS, group)
+    assert torch.equal(total, (x.float() + r.float()).to(dtype))
+    y64 = _norm64(total, w)
+    _check_codes(q, s, y64, group, DELTA["norm"])
+    q0, s0, _ = ops.add_rmsnorm_fp8_quant(total, None, w, EPS, group)
+    assert torch.equal(q0.view(torch.uint8), q.view(torch.uint8)) and torch.equal(s0, s)
+    # In place through the C ABI: the sum takes the residual's place, then x's.
+    for into in ("residual", "x"):
+        x1, r1 = x.clone(), r.clone()
+        out = r1 if into == "residual" else x1
+        q1, s1 = torch.zeros_like(q), torch.zeros_like(s)
+        status = _lib.lib().tf_add_rmsnorm_fp8_quant(
+            x1.data_ptr(), t - 1, h, h, r1.data_ptr(), h, w.data_ptr(), EPS,
+            _lib.TF_DTYPE_FP16 if dtype == torch.float16 else _lib.TF_DTYPE_BF16, group,
+            q1.data_ptr(), s1.data_ptr(), out.data_ptr(), h,
+            _lib.stream_ptr(torch.device("cuda", 0)))
+        _lib.check("tf_add_rmsnorm_fp8_quant", status)
+        assert torch.equal(out[:-1], total[:-1])
+        assert torch.equal(out[-1], (r if into == "residual" else x)[-1])
+        assert torch.equal(q1[:-1].view(torch.uint8), q[:-1].view(torch.uint8))
+        assert torch.equal(s1[:-1], s[:-1]) and not bool(s1[-1].any())
+        assert not bool(q1[-1].view(torch.uint8).any())
+
+
+# One scale a row: 1 to 4 vectors a thread, more rows than CTAs.
+@pytest.mark.parametrize("m, i", [(2500, 1000), (700, 10000), (400, 18944), (350, 32768)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_silu_of_many_rows(m: int, i: int, dtype: torch.dtype, device: torch.device) -> None:
+    gu = _stream(m, 2 * i, dtype, 3, device)
+    q, s = ops.silu_mul_fp8_quant(gu, 0)
+    g, u = gu.double().chunk(2, 1)
+    _check_codes(q, s, g / (1 + torch.exp(-g)) * u, 0, DELTA["silu"])
