@@ -245,3 +245,40 @@ def test_silu_of_many_rows(m: int, i: int, dtype: torch.dtype, device: torch.dev
     q, s = ops.silu_mul_fp8_quant(gu, 0)
     g, u = gu.double().chunk(2, 1)
     _check_codes(q, s, g / (1 + torch.exp(-g)) * u, 0, DELTA["silu"])
+
+
+# ------------------------------------------------------------------------- the choice of the form
+
+
+def _device_us(run) -> float:  # type: ignore[no-untyped-def]
+    """Device time of a call: the least of several replays of a graph of 20."""
+    run()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        for _ in range(20):
+            run()
+    graph.replay()
+    best = float("inf")
+    for _ in range(8):
+        a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+        a.record()
+        graph.replay()
+        b.record()
+        b.synchronize()
+        best = min(best, a.elapsed_time(b) * 50)
+    return best
+
+
+@pytest.mark.parametrize("n, k", [(8192, 128), (16384, 128), (37888, 128), (8192, 256),
+                                  (16384, 256), (16384, 512), (3584, 3584)])
+def test_fewer_tokens_are_not_slower(n: int, k: int, device: torch.device) -> None:
+    """Up to 512 tokens the form is chosen by an estimate, above always the CTA pairs: a call of
+    fewer tokens must not take much longer than one of 520 (320 x 8192 x 128 once took 1.6 times
+    as long)."""
+    def us(m: int) -> float:
+        args = _linear_inputs(m, n, k, torch.bfloat16, False, device)
+        return _device_us(lambda: ops.w8a8_block_linear(*args, torch.bfloat16))
+
+    most = us(520)
+    for m in (72, 128, 200, 256, 320, 512):
+        assert us(m) <= 1.25 * most, f"{m} tokens against 520 in {most:.1f} us"

@@ -975,10 +975,11 @@ int tc_prepare(TcDevice& d, TcKernel kernel, int threads, int smem, int base) {
 }
 
 // Estimated time of a launch in ns, fitted to measurements of 1 to 148 blocks of K on this GPU: a
-// fixed part (launch, set-up, first bytes from HBM, output), the exchange of a split, and a time
-// per block of the busiest cluster.
+// fixed part (launch, set-up, first bytes from HBM, output of the last tile), the exchange of a
+// split, a time per block of the busiest cluster, and one per tile of it after the first (the tile's
+// output, and the ring and the sums starting anew).
 struct TcCost {
-  int fixed, exchange, block;
+  int fixed, exchange, block, tile;
 };
 
 struct TcSplit {
@@ -991,7 +992,7 @@ struct TcSplit {
 TcSplit tc_split(const TcDevice& d, int base, const TcCost& c, const TcArgs& p) {
   const int64_t tiles = static_cast<int64_t>(p.tok_tiles) * p.w_tiles;
   const int64_t waves = cdiv(tiles, std::max(1, d.clusters[base]));
-  TcSplit best{1, c.fixed + waves * p.kb_total * c.block};
+  TcSplit best{1, c.fixed + waves * p.kb_total * c.block + (waves - 1) * c.tile};
   for (int s = 2; s * base <= 8 && s <= p.kb_total && tiles <= d.clusters[s * base]; ++s) {
     const int64_t ns = c.fixed + c.exchange + cdiv(p.kb_total, s) * c.block;
     if (ns < best.ns) best = TcSplit{s, ns};
@@ -1045,7 +1046,7 @@ bool tile_counts(const W8A8Args& a, int tokens, int rows, TcArgs* p) {
 // A kernel form: its tile counts and K split for these operands on this device, and its launch.
 template <typename T>
 struct PairForm {
-  static constexpr TcCost kCost{5400, 4600, 420};
+  static constexpr TcCost kCost{5400, 4600, 420, 1600};
   TcDevice* device;
   TcArgs p;
   int64_t ns;
@@ -1077,7 +1078,7 @@ struct PairForm {
 
 template <int kCols, typename T>
 struct SwapForm {
-  static constexpr TcCost kCost{4500, 2000, kCols == 64 ? 380 : 300};
+  static constexpr TcCost kCost{4500, 2000, kCols == 64 ? 380 : 300, 2500};
   TcDevice* device;
   TcArgs p;
   int64_t ns;
@@ -1116,7 +1117,10 @@ int run_form(const W8A8Args& a, int dev, cudaStream_t stream) {
 
 // Up to 64 tokens: one token tile with weight rows as lanes. Above, up to 512: whichever of the
 // two forms is estimated faster; 64-token tiles fill more SMs and start sooner, pairs read the
-// weights once (128 tokens: 3584 x 3584 11.9 against 13.2 us, 37888 x 3584 52 against 36).
+// weights once (128 tokens: 3584 x 3584 11.4 against 13.3 us, 37888 x 3584 50 against 36, 37888 x
+// 128 14.8 against 8.5). Of 231 products of 72 to 512 tokens, 512 to 37888 rows and K of 128 to
+// 18944, the one it takes is at most 9 % slower than the other. Without the time per tile
+// it took 64-token tiles that were up to 1.9 times slower where K is 128 or 256.
 template <typename T>
 int launch_tc(const W8A8Args& a, cudaStream_t stream) {
   int dev = 0;
