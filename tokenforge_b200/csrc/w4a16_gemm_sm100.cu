@@ -380,13 +380,9 @@ __global__ void __launch_bounds__(cta_threads<BM>(), 1)
       constexpr int kChunk = BM < 32 ? 16 : 32;
 #pragma unroll 1
       for (int c0 = 0; c0 < BM; c0 += kChunk) {
-        uint32_t r[32];
-        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(32 * q) << 16) + b * BM + c0;
-        if constexpr (kChunk == 32)
-          tmem_ld_32cols(taddr, r);
-        else
-          tmem_ld_16cols(taddr, r);
-        tmem_ld_wait();
+        uint32_t r[kChunk];
+        tmem_ld(tmem_base + (static_cast<uint32_t>(32 * q) << 16) + b * BM + c0, r);
+        tmem_ld_wait(r);
         if (w.split) {
 #pragma unroll
           for (int j = 0; j < kChunk; ++j)
