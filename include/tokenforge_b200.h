@@ -330,8 +330,10 @@ TF_API int tf_e4m3_quant_rows(const uint16_t* y, int64_t R, int64_t C, int64_t l
  *
  * These kernels are always launched as programmatic dependents of the kernel before them on the
  * stream: their CTAs may become resident before it has finished, but they access memory only
- * after it has. With TF_LAUNCH_PDL set, the norm's weight, and wq and w_scale at decode sizes,
- * are read before that, under the condition stated there. */
+ * after it has. With TF_LAUNCH_PDL set, some calls read the norm's weight (rows of 16-byte vectors,
+ * at most 32768 columns), or wq and w_scale (K at most 8192 and weights small for the number of
+ * tokens: the warp-MMA kernel), before that, under the condition stated there; all others wait
+ * first whatever the flag. */
 enum { TF_DTYPE_FP16 = 0, TF_DTYPE_BF16 = 1 };
 
 /* residual_out = dtype(x + residual);  h = residual_out in fp32;
@@ -358,8 +360,9 @@ TF_API int tf_e4m3_quant_groups(const uint16_t* x, int64_t R, int64_t C, int64_t
  * xq [M, K] row stride ldx bytes; x_scale [M, ceil(K / 128)] row stride ld_xs floats;
  * wq [N, K] contiguous; w_scale [ceil(N / 128), ceil(K / 128)] contiguous; bias dtype [N] or
  * NULL; y dtype [M, N] row stride ldy. K and ldx must be multiples of 16, xq and wq 16-byte
- * aligned; any M >= 0 and N >= 1, each size at most 2^30. No workspace; results do not depend on timing: the same call
- * gives the same bits. */
+ * aligned; any M >= 0 and N >= 1, each size at most 2^30. No workspace; results do not depend on
+ * timing: the same call gives the same bits on one GPU (how K is split depends on how many clusters
+ * of thread blocks a GPU holds at once). */
 TF_API int tf_w8a8_block_linear(const uint8_t* xq, int64_t M, int64_t K, int64_t ldx,
                                 const float* x_scale, int64_t ld_xs, const uint8_t* wq,
                                 const float* w_scale, const uint16_t* bias, int64_t N,

@@ -12,18 +12,23 @@
 // Two kernels, by which operand gives the accumulator's 128 lanes:
 //   w8a8_pair_kernel, tokens as lanes, many tokens: a CTA pair (two SMs, cta_group::2 MMAs)
 //     computes 256 tokens x 256 weight rows, each CTA holding 128 tokens' sums and half of the
-//     weight rows in shared memory, so a block costs an SM 32 KB of L2 traffic instead of the 48 KB
-//     of a single CTA's 128 x 256 tile (which stopped at 2180 TFLOP/s even without promotion). A
-//     lane is a token, so a block's scale is one number per thread, and promotion costs one
-//     packed FMA per two values. Two warps per TMEM quadrant, 128 columns each.
-//     Measured, bf16: 4096 x 37888 x 3584 in 477 us (2330 TFLOP/s; 0.50 to 0.56 ms back to back
-//     under the power cap), 1024 x 3584 x 18944 in 69 us, 256 x 3584 x 18944 in 26 us. Bound by
-//     the promotion: 840 cycles a block, where its MMAs take 512.
+//     weight rows in shared memory, so a block costs an SM 32 KB of loads instead of the 48 KB of a
+//     single CTA's 128 x 256 tile. (A kernel of such tiles stopped at 2180 TFLOP/s even without
+//     promotion. Why is not established: L2 is at a third of its throughput here.) A lane is a
+//     token, so a block's scale is one number per thread, and promotion costs one packed FMA per
+//     two values. Two warps per TMEM quadrant, 128 columns each.
+//     Measured, bf16, a graph of calls: 4096 x 37888 x 3584 in 461 to 516 us (2410 to 2160
+//     TFLOP/s, with the GPU's power state), 1024 x 37888 x 3584 in 124, 1024 x 3584 x 18944 in 67,
+//     256 x 3584 x 18944 in 27. Bound by the promotion, 847 cycles a block where its MMAs take 512
+//     (1024 x 37888 x 3584: an SM is active for 189.8 thousand cycles, 224 blocks, tile ends
+//     included), and by the clock, which falls to 1.6 GHz in that kernel and to 1.44 in a second of
+//     such calls, under the power cap.
 //   w8a8_swap_kernel, weight rows as lanes, few tokens: tile of 128 weight rows x 16, 32 or 64
 //     tokens. No tensor-core rows are wasted on missing tokens, the weight stream sets the pace,
 //     and the scale of a column (token) comes from shared memory. One warp per quadrant.
-//     Measured: 16 x 37888 x 3584 in 25.2 us (5.45 TB/s, 85 % of a copy's rate), 16 x 3584 x
-//     18944 in 17.4 us.
+//     Measured: 16 x 37888 x 3584 in 25.1 us (5.46 TB/s, 85 % of a copy's rate), 16 x 3584 x
+//     18944 in 17.4 us (28 weight tiles, 4 shares of K each: 112 of 148 SMs, since 26 clusters of 5
+//     are resident at once, and 2 us of exchange).
 //
 // Warps: 0 TMA producer, 1 TMEM allocation and MMA issue (the pair's warp 3 issues every other
 // block), 2 fetches each block's scales into a small ring; warps from 4 on promote. Persistent CTAs
