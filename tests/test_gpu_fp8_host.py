@@ -19,10 +19,10 @@ E4M3 = torch.float8_e4m3fn
 def test_outputs_that_do_not_fit_raise_out_of_memory(device: torch.device) -> None:
     """Under a limit on this process's memory, an output above it raises torch.OutOfMemoryError (a
     RuntimeError's subclass that serving code catches), from every operator."""
-    x = torch.zeros((1 << 14, 4096), dtype=torch.float16, device=device)
+    x = torch.zeros((1 << 16, 4096), dtype=torch.float16, device=device)
     w = torch.ones(4096, dtype=torch.float16, device=device)
-    xq = torch.zeros((1 << 14, 16), dtype=E4M3, device=device)
-    xs, ws = torch.ones((1 << 14, 1), device=device), torch.ones((64, 1), device=device)
+    xq = torch.zeros((1 << 16, 16), dtype=E4M3, device=device)
+    xs, ws = torch.ones((1 << 16, 1), device=device), torch.ones((64, 1), device=device)
     wq = torch.zeros((8192, 16), dtype=E4M3, device=device)
     calls = [
         lambda: ops.add_rmsnorm_fp8_quant(x, x, w, 1e-6),
@@ -48,32 +48,40 @@ def test_other_threads_run_while_a_launch_waits(device: torch.device) -> None:
     that waits for a free place must let other Python threads run, as every torch call does."""
     x = torch.zeros((1, 256), dtype=torch.float16, device=device)
     ops.e4m3_quant_groups(x)
-    gaps: list[float] = []
-    stop = threading.Event()
 
-    def tick() -> None:
-        last = time.perf_counter()
-        while not stop.is_set():
-            time.sleep(0.001)
-            now = time.perf_counter()
-            gaps.append(now - last)
-            last = now
+    def longest_gap() -> float:
+        gaps: list[float] = []
+        stop = threading.Event()
 
-    torch.cuda.synchronize()
-    thread = threading.Thread(target=tick)
-    thread.start()
-    try:
-        begin = time.perf_counter()
-        torch.cuda._sleep(800_000_000)  # cycles: 0.4 s at the highest clock, 1.965 GHz
-        for _ in range(6000):
-            ops.e4m3_quant_groups(x)
-        enqueued = time.perf_counter() - begin
+        def tick() -> None:
+            last = time.perf_counter()
+            while not stop.is_set():
+                time.sleep(0.001)
+                now = time.perf_counter()
+                gaps.append(now - last)
+                last = now
+
         torch.cuda.synchronize()
-    finally:
-        stop.set()
-        thread.join()
-    assert enqueued > 0.3, "the queue was not full: nothing waited"
-    assert max(gaps) < 0.15, f"another thread stood still for {max(gaps):.3f} s"
+        thread = threading.Thread(target=tick)
+        thread.start()
+        try:
+            begin = time.perf_counter()
+            torch.cuda._sleep(800_000_000)  # cycles: 0.4 s at the highest clock, 1.965 GHz
+            for _ in range(6000):
+                ops.e4m3_quant_groups(x)
+            enqueued = time.perf_counter() - begin
+            torch.cuda.synchronize()
+        finally:
+            stop.set()
+            thread.join()
+        assert enqueued > 0.3, "the queue was not full: nothing waited"
+        return max(gaps)
+
+    # A busy host may hold a thread up once; a launch that keeps the lock does it every time.
+    gaps = [longest_gap()]
+    while gaps[-1] > 0.15 and len(gaps) < 4:
+        gaps.append(longest_gap())
+    assert gaps[-1] <= 0.15, f"another thread stood still for {gaps} s"
 
 
 def test_without_the_extension_the_results_are_the_same(device: torch.device, monkeypatch) -> None:  # type: ignore[no-untyped-def]

@@ -48,10 +48,10 @@ def _load_fast():  # type: ignore[no-untyped-def]
     try:
         _fast = _lib.fp8_host()
     except ImportError as e:
+        _fast = _NoFastPath()
         warnings.warn(f"the FP8 operators' host fast path cannot be loaded ({e}); their calls go "
                       "through Python, 10 to 14 us each instead of 4 to 6", RuntimeWarning,
                       stacklevel=3)
-        _fast = _NoFastPath()
     return _fast
 
 
